@@ -610,6 +610,66 @@ int mq_minmax(const void* x, int32_t dtype, int64_t n, int32_t merge, double* ou
 int mq_histogram(const void* x, int32_t dtype, int64_t n, const double* edges, int32_t nbins, int64_t* counts,
                  void* hip_stream);
 
+/*
+ * Products with weights held in 4 bits: what a model does with the codes, scales and zero points that the quantizers
+ * above write.  The reference keeps such codes next to the weight (_LinearDump, quant_weight.py:876-914) and multiplies by
+ * the dequantized float16 weight; nothing in it computes on the codes, so these entry points have no counterpart there.
+ *
+ *   W[e][n][k] = scale[e][n][k / group] * (q[e][n][k] - zero[e][n][k / group])
+ *   mq_linear4       y[r]  = x[r]  W[e(r)]^T + bias[e(r)]
+ *   mq_linear4_grad  dx[r] = dy[r] W[e(r)]            (the weight is frozen: no gradient of codes or scales)
+ *   mq_bias_grad     db[e] = sum of dy[r] over the rows of e
+ *
+ * x, dy, bias: float16 or bfloat16, y / dx of the same type, sums in float32, one rounding at the end.  In mq_linear4
+ * the codes' values enter the matrix cores exactly and the scales are applied in float32.  In mq_linear4_grad the scales
+ * change along the sum, so each weight is rounded once to the type of dy (half a step: 2^-12 of it in float16, 2^-9 in
+ * bfloat16).  With zero points the sum is taken as scale * sum(q x) - scale * zero * sum(x): an infinite x[r][k] makes
+ * the whole row NaN where (q - zero) x would have left infinities.
+ *
+ * Rows and experts: counts == NULL: one weight (experts == 1) for all rows.  Otherwise the rows are sorted by expert and
+ * counts (DEVICE, int32 [experts]) says how many each has, none included; the host never reads it.  Counts below zero
+ * stand for none and the sum stops at `rows`, so no array makes a call read or write out of bounds.  Rows behind the last
+ * expert's belong to nobody: their y / dx are zero and their contents are not used.
+ */
+typedef enum {
+  MQ_W4_INT_ASYM = 0, /* unsigned codes 0 .. 15 with a zero point (_int_quant_meta(asym=True), up to 4 bits)     */
+  MQ_W4_INT_SYM = 1,  /* integers -7 .. 7 (_int_quant_meta(asym=False), up to 4 bits)                            */
+  MQ_W4_TABLE = 2,    /* sixteen table values; entry 0 must be 0; each has to be an fp8 e4m3 number, as every 3- and
+                         4-bit list of the reference is (quant_weight.py:10-31)                                  */
+  MQ_W4_FP4 = 3       /* the list FP4_E2M1 = 0, +-1, 2, 3, 4, 6, 8, 12 (quant_weight.py:22)                      */
+} mq_w4_kind;
+
+typedef struct {
+  const void* data;   /* DEVICE, 16-byte aligned, mq_w4_data_bytes: codes in tiles of 16 rows x 128 columns      */
+  const void* params; /* DEVICE, 16-byte aligned, mq_w4_params_bytes: scales (and zero points) per tile row      */
+  const float* norm;  /* DEVICE [experts]: a power of two that brings an expert's largest |weight| near 2^15; the
+                         gradient's float16 weights are held times it so that small scales keep their bits       */
+  int64_t experts, n, k;
+  int64_t group;      /* columns per scale: a multiple of 32 that divides k, or 0 = one per row (any k)          */
+  int32_t kind;       /* mq_w4_kind */
+  int32_t reserved;
+  float values[16];   /* MQ_W4_TABLE: code -> value */
+} mq_w4;
+
+size_t mq_w4_data_bytes(int64_t experts, int64_t n, int64_t k);  /* 0: refused sizes */
+size_t mq_w4_params_bytes(const mq_w4* w);                       /* 0: refused (data, params, norm not looked at) */
+/* Writes w->data and w->params.  codes [experts][n][k]: uint8 (INT_ASYM; above 15 stands for 15), int8 (INT_SYM; beyond
+ * +-7 stands for +-7) or float16 table values (TABLE, FP4; a value that is not in the table stands for 0); scale, zero:
+ * float16 [experts][n][k / group or 1], zero only with INT_ASYM. */
+int mq_w4_pack(const mq_w4* w, const void* codes, const void* scale, const void* zero, void* hip_stream);
+/* deq float16 [experts][n][k] = h(h(q - zero) * scale): the bits that the quantizers' own deq output has. */
+int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream);
+
+size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t counted, int32_t grad); /* may be 0 */
+/* x [rows][ldx] (ldx elements from row to row, 0 = the same row again), y [rows][n] contiguous, 16-byte aligned. */
+int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
+               const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream);
+int mq_linear4_grad(const mq_w4* w, const void* dy, int32_t dtype, int64_t rows, int64_t ldy, const int32_t* counts,
+                    void* dx, void* workspace, size_t workspace_bytes, void* hip_stream);
+size_t mq_bias_grad_workspace_bytes(int64_t rows, int64_t n, int64_t experts);
+int mq_bias_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ldy, int64_t experts,
+                 const int32_t* counts, void* db, void* workspace, size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,456 @@
+// Products with weights held in 4 bits (mq_linear4, mq_linear4_grad), their packing and unpacking, and the bias's
+// gradient.  Layout and decoding: mq_w4.h; the product kernels: mq_w4_kernels.h.
+//
+// MQ_W4_PART = 0: host side and the small kernels; 1 .. 8: the product kernels of one element type and kind of codes.
+#include "mq_w4_kernels.h"
+
+#ifndef MQ_W4_PART
+#define MQ_W4_PART 0
+#endif
+
+#if MQ_W4_PART == 1
+MQ_W4_LAUNCHER(w4_launch_1) { return w4_launch<W4F16, W4_S4>(a, p, pl, grad, st); }
+#elif MQ_W4_PART == 2
+MQ_W4_LAUNCHER(w4_launch_2) { return w4_launch<W4F16, W4_U4>(a, p, pl, grad, st); }
+#elif MQ_W4_PART == 3
+MQ_W4_LAUNCHER(w4_launch_3) { return w4_launch<W4F16, W4_LUT>(a, p, pl, grad, st); }
+#elif MQ_W4_PART == 4
+MQ_W4_LAUNCHER(w4_launch_4) { return w4_launch<W4F16, W4_FP4>(a, p, pl, grad, st); }
+#elif MQ_W4_PART == 5
+MQ_W4_LAUNCHER(w4_launch_5) { return w4_launch<W4BF16, W4_S4>(a, p, pl, grad, st); }
+#elif MQ_W4_PART == 6
+MQ_W4_LAUNCHER(w4_launch_6) { return w4_launch<W4BF16, W4_U4>(a, p, pl, grad, st); }
+#elif MQ_W4_PART == 7
+MQ_W4_LAUNCHER(w4_launch_7) { return w4_launch<W4BF16, W4_LUT>(a, p, pl, grad, st); }
+#elif MQ_W4_PART == 8
+MQ_W4_LAUNCHER(w4_launch_8) { return w4_launch<W4BF16, W4_FP4>(a, p, pl, grad, st); }
+#else
+
+// ---- packing ---------------------------------------------------------------------------------------
+struct PackArgs {
+  const void* codes;   // [E][N][K]: bytes, or float16 table values
+  const uint16_t* scale;
+  const uint16_t* zero;
+  uint32_t* data;
+  void* params;
+  int64_t n, k;
+  int32_t nt, kt, g, gp;  // g: groups that the scales have per row
+  float values[16];
+};
+
+// One thread per dword: eight codes of one row.  Consecutive threads take consecutive octets of a row, so that a wave
+// reads four rows' 128 bytes each.
+template <int KIND> __global__ __launch_bounds__(256) void k_w4_pack(const PackArgs p) {
+  const int t = threadIdx.x, octet = t & 15, r = t >> 4;
+  const int64_t n = (int64_t)blockIdx.y * 16 + r, k0 = (int64_t)blockIdx.x * 128 + octet * 8;
+  const int64_t e = blockIdx.z;
+  uint32_t d = 0;
+  if (n < p.n) {
+    const int64_t at = (e * p.n + n) * p.k;
+    for (int i = 0; i < 8; ++i) {
+      if (k0 + i >= p.k) break;
+      uint32_t c = 0;
+      if constexpr (KIND == W4_U4) {
+        c = static_cast<const uint8_t*>(p.codes)[at + k0 + i];
+        c = c < 15 ? c : 15;
+      } else if constexpr (KIND == W4_S4) {
+        const int v = static_cast<const int8_t*>(p.codes)[at + k0 + i];
+        const int m = v < 0 ? -v : v;
+        c = (uint32_t)(m < 7 ? m : 7) | (v < 0 ? 8u : 0u);
+      } else {
+        const float v = (float)static_cast<const half_t*>(p.codes)[at + k0 + i];
+        for (int q = 1; q < 16; ++q)
+          if (p.values[q] == v && v != 0.0f) c = q;
+      }
+      d |= w4_put<KIND>(c, i);
+    }
+  }
+  const int lane = (octet & 3) * 16 + r, j = octet >> 2;
+  p.data[((e * p.nt + blockIdx.y) * p.kt + blockIdx.x) * 256 + lane * 4 + j] = d;
+}
+__global__ __launch_bounds__(256) void k_w4_params(const PackArgs p, int64_t total) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t grp = (i >> 4) % p.gp, tile = (i >> 4) / p.gp, e = tile / p.nt, n = (tile % p.nt) * 16 + (i & 15);
+    uint32_t s = 0, z = 0;
+    if (n < p.n && grp < p.g) {
+      const int64_t at = (e * p.n + n) * p.g + grp;
+      s = p.scale[at];
+      if (p.zero) z = p.zero[at];
+    }
+    if (p.zero)
+      static_cast<uint32_t*>(p.params)[i] = s | (z << 16);
+    else
+      static_cast<uint16_t*>(p.params)[i] = (uint16_t)s;
+  }
+}
+
+// The float16 weight: h(h(q - zero) * scale), the arithmetic of the quantizers' dequantization.
+template <int KIND> __global__ __launch_bounds__(256) void k_w4_unpack(const W4Args a, uint16_t* out) {
+  const int t = threadIdx.x, octet = t & 15, r = t >> 4;
+  const int64_t n = (int64_t)blockIdx.y * 16 + r, k0 = (int64_t)blockIdx.x * 128 + octet * 8, e = blockIdx.z;
+  if (n >= a.n || k0 >= a.k) return;
+  const int64_t tile = e * a.nt + blockIdx.y;
+  const uint32_t d = a.data[(tile * a.kt + blockIdx.x) * 256 + ((octet & 3) * 16 + r) * 4 + (octet >> 2)];
+  float f[8];
+  w4_decode_f32<KIND>(d, a.lut, f);
+  const int64_t at = (tile * a.gp + w4_group(a, (int)(k0 >> 5))) * 16 + r;
+  float s, z = 0;
+  if constexpr (KIND == W4_U4) {
+    const uint32_t v = static_cast<const uint32_t*>(a.params)[at];
+    s = (float)h_from_bits(v);
+    z = (float)h_from_bits(v >> 16);
+  } else {
+    s = (float)h_from_bits(static_cast<const uint16_t*>(a.params)[at]);
+  }
+  for (int i = 0; i < 8 && k0 + i < a.k; ++i) {
+    float q = f[i] * w4_f32_scale<KIND>();
+    if constexpr (KIND == W4_U4) q = (float)h_from_bits(f2h_bits(q - z));
+    out[(e * a.n + n) * a.k + k0 + i] = (uint16_t)f2h_bits(q * s);
+  }
+}
+
+// ---- the transposed operand of the gradient ----------------------------------------------------------
+// dx = dy W contracts over the weight's rows: the same codes in the same layout with the roles of rows and columns
+// exchanged.  A thread turns 8 rows x 8 columns.  Bound by its own bytes (half a byte read and written per weight).
+template <int KIND>
+__global__ __launch_bounds__(256) void k_w4_turn(const W4Args a, uint32_t* out, int32_t ct, int32_t rb) {
+  const int t = threadIdx.x, c = t & 15, nb = t >> 4;
+  const int64_t e = blockIdx.z;
+  if (a.counts && a.counts[e] <= 0) return;
+  const int64_t nt = (int64_t)blockIdx.y * 8 + (nb >> 1);
+  uint32_t d[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    d[i] = nt < a.nt ? a.data[((e * a.nt + nt) * a.kt + blockIdx.x) * 256 + ((c & 3) * 16 + (nb & 1) * 8 + i) * 4 + (c >> 2)] : 0u;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint32_t o = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o |= w4_put<KIND>(w4_get<KIND>(d[i], q), i);
+    const int k = c * 8 + q;  // c = octet index: 4 * j + kq = (32 j + 8 kq) / 8
+    const int64_t tile = (int64_t)blockIdx.x * 8 + (k >> 4);
+    if (tile < ct) out[((e * ct + tile) * rb + blockIdx.y) * 256 + ((nb & 3) * 16 + (k & 15)) * 4 + (nb >> 2)] = o;
+  }
+}
+
+// ---- the bias's gradient -----------------------------------------------------------------------------
+// Sums of dy's rows per expert in float32: 64 columns per workgroup, an expert's rows cut into `splits` runs whose sums
+// a second launch adds in order.
+struct BiasArgs {
+  const uint16_t* dy;
+  const int32_t* counts;
+  float* part;  // [splits][E][N]
+  uint16_t* db;
+  int64_t rows, n, ldy, experts;
+  int32_t splits;
+};
+template <class T> __global__ __launch_bounds__(256) void k_w4_bias(const BiasArgs p) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + lane, e = blockIdx.z;
+  int64_t start = 0, count = p.rows;
+  if (p.counts) {
+    int64_t before = 0;
+    for (int64_t i = lane; i < e; i += 64) before += p.counts[i] > 0 ? p.counts[i] : 0;
+    for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off);
+    const int64_t c = p.counts[e] > 0 ? p.counts[e] : 0;
+    start = before < p.rows ? before : p.rows;
+    count = before + c < p.rows ? before + c - start : p.rows - start;
+  }
+  const int64_t r0 = start + count * blockIdx.y / p.splits, r1 = start + count * (blockIdx.y + 1) / p.splits;
+  float s = 0;
+  if (col < p.n) {
+#pragma unroll 4
+    for (int64_t r = r0 + w; r < r1; r += 4) s += T::to_f32(p.dy[r * p.ldy + col]);
+  }
+  red[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && col < p.n)
+    p.part[((int64_t)blockIdx.y * p.experts + e) * p.n + col] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+}
+template <class T> __global__ __launch_bounds__(256) void k_w4_bias_join(const BiasArgs p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = p.experts * p.n;
+  if (i >= total) return;
+  float s = 0;
+  for (int o = 0; o < p.splits; ++o) s += p.part[o * total + i];
+  p.db[i] = T::from_f32(s);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------
+namespace {
+
+constexpr int64_t kMaxK = 1 << 20, kMaxN = 1 << 22, kMaxExperts = 4096, kMaxRows = (int64_t)1 << 30;
+
+uint8_t e4m3_of(float v, bool* ok) {  // exact, or *ok = false
+  for (int b = 0; b < 256; ++b) {
+    if ((b & 0x7F) == 0x7F) continue;
+    const int e = b >> 3 & 15, m = b & 7;
+    float f = e ? (8 + m) * 0.125f : m * 0.125f;
+    for (int i = (e ? e : 1); i < 7; ++i) f *= 0.5f;
+    for (int i = 7; i < e; ++i) f *= 2.0f;
+    if ((b & 0x80 ? -f : f) == v && !(b == 0x80)) return (uint8_t)b;
+  }
+  *ok = false;
+  return 0;
+}
+
+int check_w4(const mq_w4* w) {
+  if (!w) return MQ_ERR_ARG;
+  if (w->experts < 1 || w->n < 1 || w->k < 1 || w->kind < 0 || w->kind > 3) return MQ_ERR_ARG;
+  if (w->experts > kMaxExperts || w->n > kMaxN || w->k > kMaxK) return MQ_ERR_TOO_LARGE;
+  if (w->group < 0) return MQ_ERR_ARG;
+  if (w->group > 0 && w->k % w->group) return MQ_ERR_GROUP;
+  if (w->group > 0 && w->group % 32) return MQ_ERR_UNSUPPORTED;
+  return MQ_OK;
+}
+int32_t steps_of_group(const mq_w4* w) { return (int32_t)(w->group > 0 ? w->group / 32 : w4_ktiles(w->k) * 4); }
+int32_t groups_padded(const mq_w4* w) {
+  const int64_t steps = w4_ktiles(w->k) * 4, gu = steps_of_group(w);
+  return (int32_t)((steps + gu - 1) / gu);
+}
+
+int fill_args(const mq_w4* w, const int32_t* counts, int64_t rows, W4Args* a) {
+  if (!w->data || !w->params || !w->norm) return MQ_ERR_ARG;
+  if ((uintptr_t)w->data % 16 || (uintptr_t)w->params % 16 || (uintptr_t)w->norm % 4 || (uintptr_t)counts % 4) return MQ_ERR_ALIGN;
+  *a = W4Args{};
+  a->data = static_cast<const uint32_t*>(w->data);
+  a->params = w->params;
+  a->norm = w->norm;
+  a->counts = counts;
+  a->experts = w->experts;
+  a->n = w->n;
+  a->k = w->k;
+  a->rows = rows;
+  a->nt = (int32_t)w4_ntiles(w->n);
+  a->kt = (int32_t)w4_ktiles(w->k);
+  a->gu = steps_of_group(w);
+  a->gp = groups_padded(w);
+  a->gmagic = a->gu > 1 ? (uint32_t)((((uint64_t)1 << 32) + a->gu - 1) / a->gu) : 0;
+  if (w->kind == W4_LUT) {
+    bool ok = true;
+    for (int i = 0; i < 16; ++i) a->lut.w[i / 4] |= (uint32_t)e4m3_of(w->values[i], &ok) << (8 * (i % 4));
+    if (!ok) return MQ_ERR_UNSUPPORTED;
+  }
+  return MQ_OK;
+}
+
+W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product* p) {
+  W4Plan pl = {};
+  const int32_t gu = steps_of_group(w);
+  pl.fs = gu % 4 == 0 ? 4 : gu % 2 == 0 ? 2 : 1;
+  p->kc = grad ? w->n : w->k;
+  p->nc = grad ? w->k : w->n;
+  p->ct = (int32_t)w4_ntiles(p->nc);
+  p->rb = (int32_t)w4_ktiles(p->kc);
+  p->splits = 1;
+  const int64_t per = counted ? (rows + w->experts - 1) / w->experts : rows;  // rows of an expert, on average
+  auto row_blocks = [&](int bm) {
+    if (!counted) return (rows + bm - 1) / bm;
+    return rows / bm + (rows < w->experts + 1 ? rows : w->experts + 1);  // every expert may end inside a tile
+  };
+  if (!grad && per <= 32) {
+    pl.mt = per <= 16 ? 1 : 2;
+    pl.nt = per > 4 && p->ct >= 2048 ? 4 : 1;
+    p->nblocks = (p->ct + pl.nt - 1) / pl.nt;
+    p->mblocks = (int32_t)row_blocks(16 * pl.mt);
+    pl.waves = 8;
+    while (pl.waves > 1 && pl.waves > p->rb) pl.waves /= 2;
+    return pl;
+  }
+  pl.bm = per <= 64 ? 64 : 128;
+  pl.bn = 128;
+  p->nblocks = (p->ct * 16 + pl.bn - 1) / pl.bn;
+  p->mblocks = (int32_t)row_blocks(pl.bm);
+  // fewer tiles than compute units: the contraction is cut, at least 4 blocks of 128 to a piece
+  const int64_t tiles = (int64_t)p->nblocks * ((rows + pl.bm - 1) / pl.bm);
+  while (p->splits < 8 && tiles * p->splits < 256 && p->rb >= 8 * p->splits) p->splits *= 2;
+  return pl;
+}
+
+size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+size_t turned_bytes(const mq_w4* w) { return (size_t)w->experts * w4_ntiles(w->k) * w4_ktiles(w->n) * 1024; }
+size_t part_bytes(const W4Product& p, int64_t rows) { return p.splits > 1 ? (size_t)p.splits * rows * p.ct * 16 * 4 : 0; }
+
+int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
+            const int32_t* counts, void* y, void* ws, size_t ws_bytes, void* stream, bool grad) {
+  int rc = check_w4(w);
+  if (rc != MQ_OK) return rc;
+  if (dtype != MQ_F16 && dtype != MQ_BF16) return MQ_ERR_UNSUPPORTED;
+  if (rows < 0 || (!counts && w->experts != 1)) return MQ_ERR_ARG;
+  if (rows > kMaxRows) return MQ_ERR_TOO_LARGE;
+  if (rows == 0) return MQ_OK;
+  const int64_t kc = grad ? w->n : w->k;
+  if (!x || !y || ldx < 0 || (ldx < kc && ldx != 0 && rows > 1)) return MQ_ERR_ARG;
+  if ((uintptr_t)x % 2 || (uintptr_t)y % 16 || (uintptr_t)bias % 2) return MQ_ERR_ALIGN;
+  W4Args a;
+  rc = fill_args(w, counts, rows, &a);
+  if (rc != MQ_OK) return rc;
+  W4Product p = {};
+  const W4Plan pl = plan_of(w, rows, grad, counts != nullptr, &p);
+  if ((int64_t)p.nblocks * p.mblocks > (int64_t)0x7FFFFFFF) return MQ_ERR_TOO_LARGE;
+  const size_t turned = grad ? up256(turned_bytes(w)) : 0;
+  const size_t need = turned + part_bytes(p, rows);
+  if (need && (!ws || ws_bytes < need)) return MQ_ERR_WORKSPACE;
+  if (need && (uintptr_t)ws % 16) return MQ_ERR_ALIGN;
+  p.x = static_cast<const uint16_t*>(x);
+  p.ldx = ldx;
+  p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
+  p.b = a.data;
+  p.bias = static_cast<const uint16_t*>(bias);
+  p.y = static_cast<uint16_t*>(y);
+  p.part = p.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(ws) + turned) : nullptr;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (grad) {
+    uint32_t* t = static_cast<uint32_t*>(ws);
+    const dim3 grid(a.kt, p.rb, (unsigned)w->experts);
+    switch (w->kind) {
+      case W4_U4: hipLaunchKernelGGL((k_w4_turn<W4_U4>), grid, dim3(256), 0, st, a, t, p.ct, p.rb); break;
+      case W4_FP4: hipLaunchKernelGGL((k_w4_turn<W4_FP4>), grid, dim3(256), 0, st, a, t, p.ct, p.rb); break;
+      default: hipLaunchKernelGGL((k_w4_turn<W4_S4>), grid, dim3(256), 0, st, a, t, p.ct, p.rb); break;  // LUT: the same bits
+    }
+    MQ_HIP(hipGetLastError());
+    p.b = t;
+  }
+  const bool h = dtype == MQ_F16;
+  hipError_t e;
+  switch (w->kind) {
+    case W4_S4: e = (h ? w4_launch_1 : w4_launch_5)(a, p, pl, grad, st); break;
+    case W4_U4: e = (h ? w4_launch_2 : w4_launch_6)(a, p, pl, grad, st); break;
+    case W4_LUT: e = (h ? w4_launch_3 : w4_launch_7)(a, p, pl, grad, st); break;
+    default: e = (h ? w4_launch_4 : w4_launch_8)(a, p, pl, grad, st); break;
+  }
+  if (e != hipSuccess) {
+    mq_set_hip_error(e, "mq_linear4");
+    return MQ_ERR_HIP;
+  }
+  return MQ_OK;
+}
+
+int32_t bias_splits(int64_t rows, int64_t experts) {
+  const int64_t s = rows / (experts < 1 ? 1 : experts) / 64;
+  return (int32_t)(s < 1 ? 1 : s > 32 ? 32 : s);
+}
+
+}  // namespace
+
+extern "C" size_t mq_w4_data_bytes(int64_t experts, int64_t n, int64_t k) {
+  if (experts < 1 || n < 1 || k < 1 || experts > kMaxExperts || n > kMaxN || k > kMaxK) return 0;
+  return (size_t)experts * w4_ntiles(n) * w4_ktiles(k) * 1024;
+}
+extern "C" size_t mq_w4_params_bytes(const mq_w4* w) {
+  if (check_w4(w) != MQ_OK) return 0;
+  return (size_t)w->experts * w4_ntiles(w->n) * groups_padded(w) * 16 * (w->kind == W4_U4 ? 4 : 2);
+}
+extern "C" int mq_w4_pack(const mq_w4* w, const void* codes, const void* scale, const void* zero, void* hip_stream) {
+  const int rc = check_w4(w);
+  if (rc != MQ_OK) return rc;
+  if (!codes || !scale || !w->data || !w->params || (zero != nullptr) != (w->kind == W4_U4)) return MQ_ERR_ARG;
+  if ((uintptr_t)w->data % 16 || (uintptr_t)w->params % 16 || (uintptr_t)scale % 2 || (uintptr_t)zero % 2 ||
+      (w->kind >= W4_LUT && (uintptr_t)codes % 2))
+    return MQ_ERR_ALIGN;
+  PackArgs p = {};
+  p.codes = codes;
+  p.scale = static_cast<const uint16_t*>(scale);
+  p.zero = static_cast<const uint16_t*>(zero);
+  p.data = static_cast<uint32_t*>(const_cast<void*>(w->data));
+  p.params = const_cast<void*>(w->params);
+  p.n = w->n;
+  p.k = w->k;
+  p.nt = (int32_t)w4_ntiles(w->n);
+  p.kt = (int32_t)w4_ktiles(w->k);
+  p.g = (int32_t)(w->group > 0 ? w->k / w->group : 1);
+  p.gp = groups_padded(w);
+  static const float fp4[16] = {0, 1, 2, 3, 4, 6, 8, 12, 0, -1, -2, -3, -4, -6, -8, -12};
+  for (int i = 0; i < 16; ++i) p.values[i] = w->kind == W4_FP4 ? fp4[i] : w->values[i];
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  for (int64_t t0 = 0; t0 < p.nt; t0 += 65535) {  // grid.y holds 65535 row tiles
+    const int64_t cnt = p.nt - t0 < 65535 ? p.nt - t0 : 65535;
+    if (cnt != p.nt && w->experts != 1) return MQ_ERR_TOO_LARGE;
+    PackArgs q = p;
+    if (cnt != p.nt) {  // one expert: a run of row tiles is a weight of its own
+      q.codes = static_cast<const char*>(codes) + t0 * 16 * p.k * (w->kind >= W4_LUT ? 2 : 1);
+      q.data = p.data + t0 * p.kt * 256;
+      q.n = p.n - t0 * 16;
+    }
+    const dim3 grid(p.kt, (unsigned)cnt, (unsigned)w->experts);
+    switch (w->kind) {
+      case W4_U4: hipLaunchKernelGGL((k_w4_pack<W4_U4>), grid, dim3(256), 0, st, q); break;
+      case W4_S4: hipLaunchKernelGGL((k_w4_pack<W4_S4>), grid, dim3(256), 0, st, q); break;
+      case W4_LUT: hipLaunchKernelGGL((k_w4_pack<W4_LUT>), grid, dim3(256), 0, st, q); break;
+      default: hipLaunchKernelGGL((k_w4_pack<W4_FP4>), grid, dim3(256), 0, st, q); break;
+    }
+    MQ_HIP(hipGetLastError());
+  }
+  const int64_t total = w->experts * p.nt * p.gp * 16, blocks = (total + 255) / 256;
+  hipLaunchKernelGGL(k_w4_params, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, p, total);
+  MQ_HIP(hipGetLastError());
+  return MQ_OK;
+}
+extern "C" int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream) {
+  int rc = check_w4(w);
+  if (rc != MQ_OK) return rc;
+  if (!deq) return MQ_ERR_ARG;
+  if ((uintptr_t)deq % 2) return MQ_ERR_ALIGN;
+  W4Args a;
+  rc = fill_args(w, nullptr, 0, &a);
+  if (rc != MQ_OK) return rc;
+  if (a.nt > 65535 && w->experts != 1) return MQ_ERR_TOO_LARGE;
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  for (int64_t t0 = 0; t0 < a.nt; t0 += 65535) {
+    const int64_t cnt = a.nt - t0 < 65535 ? a.nt - t0 : 65535;
+    W4Args b = a;
+    uint16_t* out = static_cast<uint16_t*>(deq) + t0 * 16 * a.k;
+    b.data += t0 * a.kt * 256;
+    b.params = static_cast<const char*>(a.params) + t0 * a.gp * 16 * (w->kind == W4_U4 ? 4 : 2);
+    if (w->experts == 1) b.n = a.n - t0 * 16;
+    const dim3 grid(a.kt, (unsigned)cnt, (unsigned)w->experts);
+    switch (w->kind) {
+      case W4_U4: hipLaunchKernelGGL((k_w4_unpack<W4_U4>), grid, dim3(256), 0, st, b, out); break;
+      case W4_S4: hipLaunchKernelGGL((k_w4_unpack<W4_S4>), grid, dim3(256), 0, st, b, out); break;
+      case W4_LUT: hipLaunchKernelGGL((k_w4_unpack<W4_LUT>), grid, dim3(256), 0, st, b, out); break;
+      default: hipLaunchKernelGGL((k_w4_unpack<W4_FP4>), grid, dim3(256), 0, st, b, out); break;
+    }
+    MQ_HIP(hipGetLastError());
+  }
+  return MQ_OK;
+}
+extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t counted, int32_t grad) {
+  if (check_w4(w) != MQ_OK || rows < 1 || rows > kMaxRows) return 0;
+  W4Product p = {};
+  plan_of(w, rows, grad != 0, counted != 0, &p);
+  return (grad ? up256(turned_bytes(w)) : 0) + part_bytes(p, rows);
+}
+extern "C" int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
+                          const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  return product(w, x, dtype, rows, ldx, bias, counts, y, workspace, workspace_bytes, hip_stream, false);
+}
+extern "C" int mq_linear4_grad(const mq_w4* w, const void* dy, int32_t dtype, int64_t rows, int64_t ldy,
+                               const int32_t* counts, void* dx, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  return product(w, dy, dtype, rows, ldy, nullptr, counts, dx, workspace, workspace_bytes, hip_stream, true);
+}
+extern "C" size_t mq_bias_grad_workspace_bytes(int64_t rows, int64_t n, int64_t experts) {
+  if (rows < 0 || n < 1 || experts < 1) return 0;
+  return (size_t)bias_splits(rows, experts) * experts * n * 4;
+}
+extern "C" int mq_bias_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ldy, int64_t experts,
+                            const int32_t* counts, void* db, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  if (rows < 0 || n < 1 || experts < 1 || ldy < 0 || (!counts && experts != 1) || !db || (rows > 0 && !dy)) return MQ_ERR_ARG;
+  if (dtype != MQ_F16 && dtype != MQ_BF16) return MQ_ERR_UNSUPPORTED;
+  if (rows > kMaxRows || n > kMaxN || experts > kMaxExperts) return MQ_ERR_TOO_LARGE;
+  if ((uintptr_t)dy % 2 || (uintptr_t)db % 2 || (uintptr_t)counts % 4 || (uintptr_t)workspace % 4) return MQ_ERR_ALIGN;
+  if (!workspace || workspace_bytes < mq_bias_grad_workspace_bytes(rows, n, experts)) return MQ_ERR_WORKSPACE;
+  BiasArgs p = {static_cast<const uint16_t*>(dy), counts, static_cast<float*>(workspace), static_cast<uint16_t*>(db),
+                rows, n, ldy, experts, bias_splits(rows, experts)};
+  hipStream_t st = static_cast<hipStream_t>(hip_stream);
+  const dim3 grid((unsigned)((n + 63) / 64), p.splits, (unsigned)experts), join((unsigned)((experts * n + 255) / 256));
+  if (dtype == MQ_F16) {
+    hipLaunchKernelGGL((k_w4_bias<W4F16>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_w4_bias_join<W4F16>), join, dim3(256), 0, st, p);
+  } else {
+    hipLaunchKernelGGL((k_w4_bias<W4BF16>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_w4_bias_join<W4BF16>), join, dim3(256), 0, st, p);
+  }
+  MQ_HIP(hipGetLastError());
+  return MQ_OK;
+}
+#endif

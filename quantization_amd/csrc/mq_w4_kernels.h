@@ -1,0 +1,444 @@
+// The products of one element type and one kind of 4-bit codes: k_w4_rows (few rows: bound by reading the weight),
+// k_w4_gemm (many rows: matrix cores) and their launchers.  Included by mq_linear4.hip once per (type, kind).
+//
+// Both kernels give the matrix cores the WEIGHT as the A operand and the activations as B, so a lane's four results are
+// four neighbouring output columns of one row: y is stored 8 bytes at a time.
+#pragma once
+#include "mq_w4.h"
+
+struct W4Product {
+  const uint16_t* x;     // [rows][ldx], contraction index contiguous
+  const uint32_t* b;     // packed operand: W4Args::data, or its transpose for the gradient
+  const uint16_t* bias;  // [E][nc] or NULL
+  uint16_t* y;           // [rows][nc]
+  float* part;           // [splits][rows][16 * ct] partial sums, NULL when splits == 1
+  int64_t ldx, kc, nc;   // contraction length, output columns
+  int32_t ct, rb;        // 16-column tiles of the output, 128-blocks of the contraction
+  int32_t vec;           // rows of x are 16-byte aligned and kc % 8 == 0
+  int32_t nblocks, mblocks, splits;
+};
+
+// Eight contraction-neighbours of a row of x, zeros behind the end.
+__device__ __forceinline__ u32x4 w4_load8(const uint16_t* row, int64_t k, int64_t kc, bool vec) {
+  u32x4 v = {0, 0, 0, 0};
+  if (vec) {
+    if (k < kc) v = *reinterpret_cast<const u32x4*>(row + k);
+  } else {
+    uint16_t h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = k + i < kc ? row[k + i] : (uint16_t)0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+  }
+  return v;
+}
+
+// Scales (and zero points) of the four output columns 4 * (lane / 16) .. + 3 of tile `tile` in group `grp`.
+template <int KIND>
+__device__ __forceinline__ void w4_params4(const W4Args& a, int64_t tile, int grp, int quad, f32x4& s, f32x4& sz) {
+  const int64_t at = (tile * a.gp + grp) * 16 + quad * 4;
+  if constexpr (KIND == W4_U4) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const uint32_t*>(a.params) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = (float)h_from_bits(v[i]);
+      sz[i] = s[i] * (float)h_from_bits(v[i] >> 16);  // exact: 11 x 11 bits
+    }
+  } else {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.params) + at);
+    s[0] = (float)h_from_bits(v[0]);
+    s[1] = (float)h_from_bits(v[0] >> 16);
+    s[2] = (float)h_from_bits(v[1]);
+    s[3] = (float)h_from_bits(v[1] >> 16);
+  }
+}
+
+template <class T> __device__ __forceinline__ void w4_store4(uint16_t* y, int64_t nc, int64_t row, int64_t col, f32x4 v) {
+  uint16_t* to = y + row * nc + col;
+  if (nc % 4 == 0) {  // (y itself is 16-byte aligned)
+    u32x2 o;
+    o[0] = T::pack(v[0], v[1]);
+    o[1] = T::pack(v[2], v[3]);
+    *reinterpret_cast<u32x2*>(to) = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < nc) to[i] = T::from_f32(v[i]);
+  }
+}
+template <class T>
+__device__ __forceinline__ f32x4 w4_bias4(const uint16_t* bias, int64_t nc, int expert, int64_t col, f32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i < nc) v[i] += T::to_f32(bias[expert * nc + col + i]);
+  return v;
+}
+
+// ---- few rows --------------------------------------------------------------------------------------
+// A workgroup owns NT column tiles and 16 * MT rows; its waves take the 128-blocks of the contraction in turn and their
+// sums meet in LDS at the end, in the waves' order.
+template <class T, int KIND, int MT, int NT, int FS>
+__global__ __launch_bounds__(512) void k_w4_rows(const W4Args a, const W4Product p) {
+  extern __shared__ f32x4 w4_red[];
+  constexpr int D = MT * NT >= 4 ? 1 : 2;  // 128-blocks in flight per wave
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int quad = lane >> 4;
+  const int64_t tile0 = (int64_t)(blockIdx.x % p.nblocks) * NT;
+  int expert, rows;
+  int64_t row0;
+  if (!w4_find_tile(a, 16 * MT, blockIdx.x / p.nblocks, expert, row0, rows)) return;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = {0, 0, 0, 0};
+
+  if (expert >= 0) {
+    int64_t tile[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) tile[n] = (int64_t)expert * a.nt + (tile0 + n < a.nt ? tile0 + n : a.nt - 1);
+    const uint16_t* xr[MT];
+    bool live[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = m * 16 + (lane & 15);
+      live[m] = r < rows;
+      xr[m] = p.x + (row0 + (live[m] ? r : 0)) * p.ldx;
+    }
+    for (int kb = w; kb < a.kt; kb += nw * D) {
+      u32x4 wv[D][NT], xv[D][MT][4];
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int k0 = kb + d * nw;
+        if (k0 < a.kt) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) wv[d][n] = *reinterpret_cast<const u32x4*>(p.b + (tile[n] * a.kt + k0) * 256 + lane * 4);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              xv[d][m][j] = {0, 0, 0, 0};
+              if (live[m]) xv[d][m][j] = w4_load8(xr[m], (int64_t)k0 * 128 + j * 32 + quad * 8, p.kc, p.vec);
+            }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int k0 = kb + d * nw;
+        if (k0 < a.kt) {
+          f32x4 tmp[MT][NT], xs[MT];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j % FS == 0) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                xs[m] = {0, 0, 0, 0};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) tmp[m][n] = {0, 0, 0, 0};
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const u32x4 v = w4_decode<T, KIND>(wv[d][n][j], a.lut);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) tmp[m][n] = T::mfma(v, xv[d][m][j], tmp[m][n]);
+            }
+            if constexpr (KIND == W4_U4) {
+              const u32x4 ones = {T::kOnes, T::kOnes, T::kOnes, T::kOnes};
+#pragma unroll
+              for (int m = 0; m < MT; ++m) xs[m] = T::mfma(ones, xv[d][m][j], xs[m]);
+            }
+            if ((j + 1) % FS == 0) {
+              const int grp = w4_group(a, k0 * 4 + j);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                f32x4 s, sz;
+                w4_params4<KIND>(a, tile[n], grp, quad, s, sz);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    acc[m][n][i] = __builtin_fmaf(s[i], tmp[m][n][i], acc[m][n][i]);
+                    if constexpr (KIND == W4_U4) acc[m][n][i] = __builtin_fmaf(-sz[i], xs[m][i], acc[m][n][i]);
+                  }
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) w4_red[((w * MT + m) * NT + n) * 64 + lane] = acc[m][n];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * NT * 64; i += blockDim.x) {
+    f32x4 v = w4_red[i];
+    for (int o = 1; o < nw; ++o) v += w4_red[o * MT * NT * 64 + i];
+    const int l = i & 63, n = (i >> 6) % NT, m = (i >> 6) / NT;
+    const int r = m * 16 + (l & 15);
+    const int64_t col = (tile0 + n) * 16 + (l >> 4) * 4;
+    if (r < rows && col < p.nc) {
+      if (p.bias && expert >= 0) v = w4_bias4<T>(p.bias, p.nc, expert, col, v);
+      w4_store4<T>(p.y, p.nc, row0 + r, col, v);
+    }
+  }
+}
+
+// ---- many rows -------------------------------------------------------------------------------------
+// A workgroup of WM x WN waves owns 16 MT WM rows and 16 NT WN columns.  A 128-block of the rows is staged in LDS in
+// operand order (1 KiB per 16 rows x 32 contraction indices: lane l's 16 bytes at 16 l, so every access is one wave's
+// contiguous KiB), the packed weight goes from memory straight into the registers of the wave that decodes it.
+// GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.
+// GRAD = true (dx = dy W, operand b transposed): scales change along the contraction, so they are multiplied into the
+// weights, which are rounded once to T -- half a step of T per weight, as a weight stored in T has.
+template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int FS>
+__global__ __launch_bounds__(64 * WM * WN) void k_w4_gemm(const W4Args a, const W4Product p) {
+  constexpr int BM = 16 * MT * WM, NW = WM * WN, CH = BM / 16 * 4 / NW;  // 1 KiB pieces per wave
+  static_assert(BM / 16 * 4 % NW == 0, "pieces of a block are dealt evenly");
+  __shared__ u32x4 lds[2][BM / 16 * 4 * 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, quad = lane >> 4;
+  const int wm = w % WM, wn = w / WM;
+  const int64_t mb = blockIdx.x % p.mblocks;
+  const int64_t tile0 = ((int64_t)(blockIdx.x / p.mblocks) * WN + wn) * NT;
+  int expert, rows;
+  int64_t row0;
+  if (!w4_find_tile(a, BM, mb, expert, row0, rows)) return;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = {0, 0, 0, 0};
+
+  if (expert >= 0) {
+    int64_t tile[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) tile[n] = (int64_t)expert * p.ct + (tile0 + n < p.ct ? tile0 + n : p.ct - 1);
+    const int kb0 = (int)((int64_t)p.rb * blockIdx.y / p.splits), kb1 = (int)((int64_t)p.rb * (blockIdx.y + 1) / p.splits);
+    u32x4 xn[CH], wn4[NT];
+    auto load = [&](int kb) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int piece = w * CH + c;
+        const int r = (piece >> 2) * 16 + (lane & 15);
+        const int64_t k = (int64_t)kb * 128 + (piece & 3) * 32 + quad * 8;
+        xn[c] = w4_load8(p.x + (row0 + (r < rows ? r : rows - 1)) * p.ldx, k, p.kc, p.vec);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) wn4[n] = *reinterpret_cast<const u32x4*>(p.b + (tile[n] * p.rb + kb) * 256 + lane * 4);
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) lds[buf][(w * CH + c) * 64 + lane] = xn[c];
+    };
+    if (kb0 < kb1) {
+      load(kb0);
+      put(0);
+    }
+    __syncthreads();
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int buf = (kb - kb0) & 1;
+      u32x4 wv[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) wv[n] = wn4[n];
+      if (kb + 1 < kb1) load(kb + 1);
+      const u32x4* xb = lds[buf] + wm * MT * 4 * 64 + lane;
+      if constexpr (!GRAD) {
+        f32x4 tmp[MT][NT], xs[MT];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j % FS == 0) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              xs[m] = {0, 0, 0, 0};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) tmp[m][n] = {0, 0, 0, 0};
+            }
+          }
+          u32x4 xv[MT];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) xv[m] = xb[(m * 4 + j) * 64];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const u32x4 v = w4_decode<T, KIND>(wv[n][j], a.lut);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) tmp[m][n] = T::mfma(v, xv[m], tmp[m][n]);
+          }
+          if constexpr (KIND == W4_U4) {
+            const u32x4 ones = {T::kOnes, T::kOnes, T::kOnes, T::kOnes};
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xs[m] = T::mfma(ones, xv[m], xs[m]);
+          }
+          if ((j + 1) % FS == 0) {
+            const int grp = w4_group(a, kb * 4 + j);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              f32x4 s, sz;
+              w4_params4<KIND>(a, tile[n], grp, quad, s, sz);
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  acc[m][n][i] = __builtin_fmaf(s[i], tmp[m][n][i], acc[m][n][i]);
+                  if constexpr (KIND == W4_U4) acc[m][n][i] = __builtin_fmaf(-sz[i], xs[m][i], acc[m][n][i]);
+                }
+            }
+          }
+        }
+      } else {
+        constexpr int SETS = FS == 1 ? (NT + 1) / 2 : 1;  // groups under a wave's 16 NT columns
+        const float up = a.norm[expert];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float s[SETS][8], sz[SETS][8];
+          const int64_t n0 = (int64_t)kb * 128 + j * 32 + quad * 8;
+          const int64_t nt = (int64_t)expert * a.nt + (n0 / 16 < a.nt ? n0 / 16 : a.nt - 1);
+#pragma unroll
+          for (int g = 0; g < SETS; ++g) {
+            const int64_t c = tile0 + 2 * g < p.ct ? tile0 + 2 * g : p.ct - 1;
+            const int64_t at = (nt * a.gp + w4_group(a, (int)(c >> 1))) * 16 + (n0 & 8);
+            if constexpr (KIND == W4_U4) {
+              const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const uint32_t*>(a.params) + at);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const u32x4 v = q[h];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  s[g][4 * h + i] = (float)h_from_bits(v[i]) * up;
+                  sz[g][4 * h + i] = s[g][4 * h + i] * (float)h_from_bits(v[i] >> 16);
+                }
+              }
+            } else {
+              const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.params) + at);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                s[g][2 * i] = (float)h_from_bits(v[i]) * up;
+                s[g][2 * i + 1] = (float)h_from_bits(v[i] >> 16) * up;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[g][i] *= w4_f32_scale<KIND>();
+          }
+          u32x4 xv[MT];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) xv[m] = xb[(m * 4 + j) * 64];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float f[8];
+            w4_decode_f32<KIND>(wv[n][j], a.lut, f);
+            constexpr int per = FS == 1 ? 2 : NT;
+            const int g = n / per;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              f[i] = KIND == W4_U4 ? __builtin_fmaf(f[i], s[g][i], -sz[g][i]) : f[i] * s[g][i];
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = T::pack(f[2 * i], f[2 * i + 1]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m][n] = T::mfma(v, xv[m], acc[m][n]);
+          }
+        }
+      }
+      if (kb + 1 < kb1) put(buf ^ 1);
+      __syncthreads();
+    }
+    if constexpr (GRAD) {
+      const float down = 1.0f / a.norm[expert];  // a power of two
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] *= down;
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = (wm * MT + m) * 16 + (lane & 15);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int64_t col = (tile0 + n) * 16 + quad * 4;
+      if (r < rows && col < p.nc) {
+        f32x4 v = acc[m][n];
+        if (p.bias && expert >= 0 && blockIdx.y == 0) v = w4_bias4<T>(p.bias, p.nc, expert, col, v);
+        if (p.part)
+          *reinterpret_cast<f32x4*>(p.part + ((int64_t)blockIdx.y * a.rows + row0 + r) * (p.ct * 16) + col) = v;
+        else
+          w4_store4<T>(p.y, p.nc, row0 + r, col, v);
+      }
+    }
+  }
+}
+
+// The splits' partial sums, added in their order.
+template <class T> __global__ __launch_bounds__(256) void k_w4_join(const W4Product p, int64_t rows) {
+  const int64_t quads = (int64_t)p.ct * 4, total = rows * quads;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / quads, col = (i % quads) * 4;
+    if (col >= p.nc) continue;
+    const f32x4* from = reinterpret_cast<const f32x4*>(p.part) + i;
+    f32x4 v = from[0];
+    for (int s = 1; s < p.splits; ++s) v += from[s * total];
+    w4_store4<T>(p.y, p.nc, row, col, v);
+  }
+}
+
+// ---- launchers: one set per (type, kind) -------------------------------------------------------------
+struct W4Plan {
+  int mt, nt, waves;  // k_w4_rows
+  int bm, bn;         // k_w4_gemm (bm = 0: k_w4_rows)
+  int fs;
+};
+
+template <class T, int KIND, int MT, int NT>
+static void w4_rows_go(const W4Args& a, const W4Product& p, const W4Plan& pl, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)p.nblocks * p.mblocks)), block(64 * pl.waves);
+  const size_t lds = (size_t)pl.waves * MT * NT * 1024;
+  if (pl.fs == 4)
+    hipLaunchKernelGGL((k_w4_rows<T, KIND, MT, NT, 4>), grid, block, lds, st, a, p);
+  else if (pl.fs == 2)
+    hipLaunchKernelGGL((k_w4_rows<T, KIND, MT, NT, 2>), grid, block, lds, st, a, p);
+  else
+    hipLaunchKernelGGL((k_w4_rows<T, KIND, MT, NT, 1>), grid, block, lds, st, a, p);
+}
+template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN>
+static void w4_gemm_go(const W4Args& a, const W4Product& p, const W4Plan& pl, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)p.nblocks * p.mblocks), p.splits), block(64 * WM * WN);
+  if (GRAD ? pl.fs >= 2 : pl.fs == 4)
+    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, 4>), grid, block, 0, st, a, p);
+  else if (!GRAD && pl.fs == 2)
+    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, GRAD ? 4 : 2>), grid, block, 0, st, a, p);
+  else
+    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, 1>), grid, block, 0, st, a, p);
+}
+
+template <class T, int KIND>
+hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool grad, hipStream_t st) {
+  if (!pl.bm) {
+    if (pl.mt == 1 && pl.nt == 1) w4_rows_go<T, KIND, 1, 1>(a, p, pl, st);
+    else if (pl.mt == 1) w4_rows_go<T, KIND, 1, 4>(a, p, pl, st);
+    else if (pl.nt == 1) w4_rows_go<T, KIND, 2, 1>(a, p, pl, st);
+    else w4_rows_go<T, KIND, 2, 4>(a, p, pl, st);
+  } else if (grad) {
+    if (pl.bm == 64) w4_gemm_go<T, KIND, true, 2, 4, 2, 2>(a, p, pl, st);
+    else w4_gemm_go<T, KIND, true, 4, 4, 2, 2>(a, p, pl, st);
+  } else {
+    if (pl.bm == 64) w4_gemm_go<T, KIND, false, 2, 4, 2, 2>(a, p, pl, st);
+    else w4_gemm_go<T, KIND, false, 4, 4, 2, 2>(a, p, pl, st);
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !p.part) return e;
+  const int64_t work = (a.rows * p.ct * 4 + 255) / 256;
+  hipLaunchKernelGGL((k_w4_join<T>), dim3((unsigned)(work < 2048 ? work : 2048)), dim3(256), 0, st, p, a.rows);
+  return hipGetLastError();
+}
+
+// The eight instances live in objects of their own (mq_linear4.hip with MQ_W4_PART = 1 .. 8).
+#define MQ_W4_LAUNCHER(NAME) hipError_t NAME(const W4Args& a, const W4Product& p, const W4Plan& pl, bool grad, hipStream_t st)
+MQ_W4_LAUNCHER(w4_launch_1);
+MQ_W4_LAUNCHER(w4_launch_2);
+MQ_W4_LAUNCHER(w4_launch_3);
+MQ_W4_LAUNCHER(w4_launch_4);
+MQ_W4_LAUNCHER(w4_launch_5);
+MQ_W4_LAUNCHER(w4_launch_6);
+MQ_W4_LAUNCHER(w4_launch_7);
+MQ_W4_LAUNCHER(w4_launch_8);

@@ -1,0 +1,392 @@
+"""Products with weights held in 4 bits: the codes, scales and zero points of quant_weight's quantizers, packed into the
+layout that the matrix-core kernels read (include/mq.h, mq_w4 / mq_linear4), and the products on them.
+
+  pack_weight(w, wq_bits, datatype, group_size)      quantize a weight [N, K] (or experts [E, N, K]) and pack it
+  pack_codes(q, scale, zp, wq_bits, datatype, ...)   pack what _int_quant_meta / _fp_quant_meta returned
+  packed_linear(x, weight, bias)                     x W^T + bias, any number of rows; backward: dx, db
+  packed_expert_linear(x, weight, counts, bias)      the same with rows sorted by expert; backward: dx, db
+  PackedLinear                                       nn.Linear's place in a model (quant_model(..., packed=True))
+
+W = scale * (q - zero point), per group of input channels; the weight is frozen (no gradient for codes or scales).
+Activations are float16 or bfloat16, sums float32, results rounded once.  The reference keeps such codes beside the weight
+(_LinearDump, quant_weight.py:876-914) and multiplies by the dequantized float16 weight; there is no CPU compute path.
+"""
+import ctypes
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .fused import TABLE_LISTS, lut_values, require_device
+
+INT_ASYM, INT_SYM, TABLE, FP4 = 0, 1, 2, 3   # mq_w4_kind
+_XDTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+class _W4(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("params", ctypes.c_void_p), ("norm", ctypes.c_void_p),
+                ("experts", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64), ("group", ctypes.c_int64),
+                ("kind", ctypes.c_int32), ("reserved", ctypes.c_int32), ("values", ctypes.c_float * 16)]
+
+
+_bound = None
+
+
+def _bind():
+    """libmq.so with the signatures of the 4-bit entry points set."""
+    global _bound
+    if _bound is None:
+        L = _lib.lib()
+        vp, i64, i32, sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
+        pw = ctypes.POINTER(_W4)
+        L.mq_w4_data_bytes.restype, L.mq_w4_data_bytes.argtypes = sz, [i64, i64, i64]
+        L.mq_w4_params_bytes.restype, L.mq_w4_params_bytes.argtypes = sz, [pw]
+        L.mq_w4_pack.restype, L.mq_w4_pack.argtypes = ctypes.c_int, [pw, vp, vp, vp, vp]
+        L.mq_w4_unpack.restype, L.mq_w4_unpack.argtypes = ctypes.c_int, [pw, vp, vp]
+        L.mq_linear4_workspace_bytes.restype, L.mq_linear4_workspace_bytes.argtypes = sz, [pw, i64, i32, i32]
+        L.mq_linear4.restype, L.mq_linear4.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, vp, sz, vp]
+        L.mq_linear4_grad.restype, L.mq_linear4_grad.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, sz, vp]
+        L.mq_bias_grad_workspace_bytes.restype, L.mq_bias_grad_workspace_bytes.argtypes = sz, [i64, i64, i64]
+        L.mq_bias_grad.restype, L.mq_bias_grad.argtypes = ctypes.c_int, [vp, i32, i64, i64, i64, i64, vp, vp, vp, sz, vp]
+        _bound = L
+    return _bound
+
+
+def table_order(values):
+    """The sixteen entries of a 3- / 4-bit value list by code: 0 and the positive values, then (from entry 9) the
+    negative ones; an eighth value of one sign stands in entry 8."""
+    pos, neg = sorted(v for v in values if v > 0), sorted((v for v in values if v < 0), reverse=True)
+    if len(pos) > 8 or len(neg) > 8 or len(pos) + len(neg) > 15:
+        raise ValueError("a 4-bit table holds at most 16 values")
+    out = [0.0] * 16
+    out[1:1 + len(pos[:7])] = pos[:7]
+    out[9:9 + len(neg[:7])] = neg[:7]
+    if len(pos) + len(neg) == 15:
+        out[8] = (pos + neg)[7] if len(pos) == 8 else neg[7]
+    return out
+
+
+def _kind_of(wq_bits, datatype):
+    """-> (mq_w4_kind, table by code | None); the refusals of quant_datatype for names it does not know
+    (quant_weight.py:553-556)."""
+    from .quant_weight import _KNOWN_TABLES
+    if not isinstance(datatype, str):
+        raise ValueError(f"unexpected data type {datatype!r}.")
+    if datatype.startswith("int"):
+        if wq_bits not in (2, 3, 4):
+            raise ValueError(f"packed weights hold 2-, 3- or 4-bit integers, not {wq_bits}-bit")
+        return (INT_ASYM if "asym" in datatype else INT_SYM), None
+    if wq_bits not in (3, 4):
+        raise ValueError(f"packed weights hold 3- or 4-bit tables, not {wq_bits}-bit")
+    if datatype not in _KNOWN_TABLES[wq_bits]:
+        raise ValueError(f"unexpected data type {datatype}.")
+    if datatype == "fp4":
+        return FP4, None
+    return TABLE, table_order(TABLE_LISTS[datatype] if datatype in TABLE_LISTS else lut_values(datatype))
+
+
+def _group(group_size):
+    """quant_weight.py:241-255: > 0 per group, -1 per tensor, everything else per row."""
+    if group_size is None or (group_size <= 0 and group_size != -1):
+        return 0
+    return int(group_size)
+
+
+class PackedWeight:
+    """A weight [N, K], or a stack of experts [E, N, K], held in 4 bits on a ROCm device.
+
+    data, params, norm: what the kernels read (include/mq.h, mq_w4), all integer tensors, so that no module-wide change
+    of dtype touches them.  experts: E, or None for a single weight."""
+
+    def __init__(self, data, params, norm, experts, n, k, group_size, wq_bits, datatype):
+        self.data, self.params, self.norm = data, params, norm
+        self.experts, self.n, self.k = experts, int(n), int(k)
+        self.group_size, self.wq_bits, self.datatype = _group(group_size), wq_bits, datatype
+        self._describe()
+
+    def _describe(self):
+        kind, values = _kind_of(self.wq_bits, self.datatype)
+        s = _W4(data=self.data.data_ptr() or None, params=self.params.data_ptr() or None, norm=self.norm.data_ptr() or None,
+                experts=self.experts or 1, n=self.n, k=self.k, group=max(self.group_size, 0), kind=kind)
+        if values is not None:
+            s.values[:] = values
+        self._c = s
+        self._ref = ctypes.byref(s)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._describe()
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def shape(self):
+        return torch.Size((self.n, self.k) if self.experts is None else (self.experts, self.n, self.k))
+
+    def to(self, device):
+        """The same weight on another ROCm device."""
+        return PackedWeight(self.data.to(device), self.params.to(device), self.norm.to(device), self.experts, self.n, self.k,
+                            self.group_size, self.wq_bits, self.datatype)
+
+    @torch.no_grad()
+    def dequantize(self):
+        """The float16 weight, with the bits that quant_int / quant_int_asym / quant_datatype return for it."""
+        out = torch.empty(self.shape, dtype=torch.float16, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(_bind().mq_w4_unpack(self._ref, out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        return out
+
+    def __repr__(self):
+        g = {0: "per row", -1: "per tensor"}.get(self.group_size, f"groups of {self.group_size}")
+        return f"PackedWeight({tuple(self.shape)}, {self.wq_bits}-bit {self.datatype}, {g}, {self.device})"
+
+
+@torch.no_grad()
+def pack_codes(q, scale, zp=None, wq_bits: int = 4, datatype: str = "int4", group_size=None) -> PackedWeight:
+    """Pack codes and parameters as _int_quant_meta / _fp_quant_meta return them (quant_weight.py:717-872).
+
+    q: int8 / uint8 codes (integers) or float16 table values, [N, K] or [N, G, group_size]; scale (and, for asymmetric
+    integers, zp): float16, [N, G] per group, [N] per row, [] per tensor.  With a leading dimension E on all of them: a
+    stack of experts.  Groups are multiples of 32 that divide K; rows may have any length."""
+    kind, values = _kind_of(wq_bits, datatype)
+    g = _group(group_size)
+    experts = scale.dim() - (2 if g > 0 else 0 if g == -1 else 1)
+    if experts not in (0, 1):
+        raise ValueError(f"scale: {tuple(scale.shape)} is no shape of scales for group_size {group_size}")
+    lead = tuple(scale.shape[:experts])
+    if q.dim() == experts + 3 and g > 0:
+        q = q.flatten(-2)
+    if q.dim() != experts + 2 or tuple(q.shape[:experts]) != lead:
+        raise ValueError(f"codes {tuple(q.shape)} and scales {tuple(scale.shape)} do not belong together")
+    n, k = q.shape[-2:]
+    if min(q.shape) < 1:
+        raise ValueError(f"an empty weight {tuple(q.shape)} cannot be packed")
+    if g > 0 and k % g:
+        raise RuntimeError(f"shape '[{n}, {k // g}, {g}]' is invalid for input of size {n * k}")
+    if g > 0 and g % 32:
+        raise ValueError(f"packed weights have groups of a multiple of 32 input channels, not {g}")
+    want = lead + ((n, k // g) if g > 0 else () if g == -1 else (n,))
+    if (zp is not None) != (kind == INT_ASYM):
+        raise ValueError(f"{datatype}: a zero point goes with asymmetric integers, and only with them")
+    for name, t in (("scale", scale), ("zp", zp)):
+        if t is not None and (tuple(t.shape) != want or t.dtype != torch.float16):
+            raise ValueError(f"{name}: float16 {want} wanted, got {t.dtype} {tuple(t.shape)}")
+    if q.dtype not in ((torch.float16,) if kind >= TABLE else (torch.int8, torch.uint8)):
+        raise ValueError(f"codes of {datatype} cannot be {q.dtype}")
+    q = require_device(q).contiguous()
+    dev = q.device
+
+    def rows(t):   # one scale per row at least
+        t = t.to(dev)
+        if g == -1:
+            t = t.reshape(lead + (1,)).expand(lead + (n,))
+        return t.contiguous()
+
+    scale, zp = rows(scale), None if zp is None else rows(zp)
+    L = _bind()
+    e = lead[0] if experts else 1
+    c = _W4(experts=e, n=n, k=k, group=max(g, 0), kind=kind)
+    if values is not None:
+        c.values[:] = values
+    nbytes, pbytes = L.mq_w4_data_bytes(e, n, k), L.mq_w4_params_bytes(ctypes.byref(c))
+    if not nbytes or not pbytes:
+        raise ValueError(f"a weight of {tuple(q.shape)} is beyond what can be packed")
+    # a power of two that brings the largest |weight| below 2^15 and above 2^13 (gradient of float16 activations)
+    top = scale.reshape(e, -1).abs().amax(1).float()
+    reach = 15 + zp.reshape(e, -1).abs().amax(1).float() if zp is not None else 16.0
+    exponent = torch.frexp(top * reach).exponent
+    ok = torch.isfinite(top * reach) & (top > 0)
+    norm = (127 + torch.where(ok, 15 - exponent, torch.zeros_like(exponent))) << 23   # the bits of 2^(15 - exponent)
+    data = torch.empty(nbytes // 4, dtype=torch.int32, device=dev)
+    params = torch.empty(pbytes // 2, dtype=torch.int16, device=dev)
+    c.data, c.params = data.data_ptr(), params.data_ptr()
+    with torch.cuda.device(dev):
+        _lib.check(L.mq_w4_pack(ctypes.byref(c), q.data_ptr(), scale.data_ptr(), None if zp is None else zp.data_ptr(),
+                                torch.cuda.current_stream().cuda_stream))
+    return PackedWeight(data, params, norm.to(torch.int32), lead[0] if experts else None, n, k, group_size, wq_bits,
+                        datatype)
+
+
+@torch.no_grad()
+def pack_weight(w, wq_bits: int = 4, datatype: str = "int4", group_size=None) -> PackedWeight:
+    """Quantize a weight [N, K] or a stack of experts [E, N, K] with the quantizers of quant_weight and pack the result."""
+    from .quant_weight import _fp_quant_meta, _int_quant_meta
+    kind, _ = _kind_of(wq_bits, datatype)
+    if w.dim() not in (2, 3):
+        raise ValueError(f"a weight [N, K] or [E, N, K] is wanted, got {tuple(w.shape)}")
+    if min(w.shape) < 1:
+        raise ValueError(f"an empty weight {tuple(w.shape)} cannot be packed")
+    g = _group(group_size)
+    if g > 0 and w.shape[-1] % g == 0 and g % 32:
+        raise ValueError(f"packed weights have groups of a multiple of 32 input channels, not {g}")
+
+    def meta(m):
+        if kind >= TABLE:
+            _, q, scale = _fp_quant_meta(m, wq_bits=wq_bits, datatype=datatype, group_size=group_size)
+            return q, scale, None
+        _, q, scale, zp = _int_quant_meta(m, wq_bits=wq_bits, asym=kind == INT_ASYM, group_size=group_size)
+        return q, scale, zp
+
+    w = require_device(w)
+    if w.dim() == 2:
+        q, scale, zp = meta(w)
+    elif g == -1:   # one scale per expert
+        parts = [meta(m) for m in w]
+        q, scale = torch.stack([p[0] for p in parts]), torch.stack([p[1] for p in parts])
+        zp = torch.stack([p[2] for p in parts]) if kind == INT_ASYM else None
+    else:
+        e, n, k = w.shape
+        q, scale, zp = meta(w.reshape(e * n, k))
+        q, scale = q.reshape(e, n, k), scale.reshape((e, n) + tuple(scale.shape[1:]))
+        zp = None if zp is None else zp.reshape(scale.shape)
+    return pack_codes(q, scale, zp, wq_bits, datatype, group_size)
+
+
+def _rows_of(t):
+    """A 2-D tensor as (tensor, elements from row to row) with neighbouring columns side by side."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and 0 < t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _product(t, weight, bias, counts, grad):
+    """One launch of mq_linear4 (grad: mq_linear4_grad) on rows t [R, K] ([R, N])."""
+    L = _bind()
+    rows = t.shape[0]
+    out = torch.empty(rows, weight.k if grad else weight.n, dtype=t.dtype, device=t.device)
+    if not rows:
+        return out
+    t, ld = _rows_of(t)
+    cp = None if counts is None else counts.data_ptr()
+    with torch.cuda.device(t.device):
+        need = L.mq_linear4_workspace_bytes(weight._ref, rows, counts is not None, grad)
+        # of this call alone: a captured graph keeps it in its own pool, and calls on other streams have their own
+        ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
+        wp = None if ws is None else ws.data_ptr()
+        stream = torch.cuda.current_stream().cuda_stream
+        if grad:
+            rc = L.mq_linear4_grad(weight._ref, t.data_ptr(), _XDTYPES[t.dtype], rows, ld, cp, out.data_ptr(), wp, need, stream)
+        else:
+            rc = L.mq_linear4(weight._ref, t.data_ptr(), _XDTYPES[t.dtype], rows, ld, None if bias is None else bias.data_ptr(),
+                              cp, out.data_ptr(), wp, need, stream)
+    _lib.check(rc)
+    return out
+
+
+def _bias_grad(dy, experts, counts):
+    L = _bind()
+    rows, n = dy.shape
+    db = torch.empty((n,) if experts is None else (experts, n), dtype=dy.dtype, device=dy.device)
+    dy, ld = _rows_of(dy)
+    with torch.cuda.device(dy.device):
+        need = L.mq_bias_grad_workspace_bytes(rows, n, experts or 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
+        _lib.check(L.mq_bias_grad(dy.data_ptr() or None, _XDTYPES[dy.dtype], rows, n, ld, experts or 1,
+                                  None if counts is None else counts.data_ptr(), db.data_ptr(), ws.data_ptr(), need,
+                                  torch.cuda.current_stream().cuda_stream))
+    return db
+
+
+class _PackedProduct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, weight, counts):
+        ctx.weight = weight
+        ctx.save_for_backward(counts)
+        return _product(x, weight, bias, counts, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (counts,), weight = ctx.saved_tensors, ctx.weight
+        dx = _product(dy, weight, None, counts, True) if ctx.needs_input_grad[0] else None
+        db = _bias_grad(dy, weight.experts, counts) if ctx.needs_input_grad[1] else None
+        return dx, db, None, None
+
+
+def _check_operands(x, weight, bias):
+    if not isinstance(weight, PackedWeight):
+        raise TypeError(f"a PackedWeight is wanted, got {type(weight).__name__}")
+    if not x.is_cuda:
+        raise RuntimeError("packed products expect ROCm device tensors; no CPU fallback exists")
+    if x.dtype not in _XDTYPES:
+        raise ValueError(f"float16 or bfloat16 activations are wanted, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != weight.k:
+        raise ValueError(f"activations {tuple(x.shape)} do not fit a weight {tuple(weight.shape)}")
+    if x.device != weight.device:
+        raise ValueError(f"activations on {x.device}, weight on {weight.device}")
+    if bias is not None:
+        want = (weight.n,) if weight.experts is None else (weight.experts, weight.n)
+        if tuple(bias.shape) != want or bias.dtype != x.dtype or bias.device != x.device:
+            raise ValueError(f"bias: {x.dtype} {want} on {x.device} wanted, got {bias.dtype} {tuple(bias.shape)} on "
+                             f"{bias.device}")
+        bias = bias.contiguous()
+    return bias
+
+
+def _run(x, weight, bias, counts):
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        return _PackedProduct.apply(x, bias, weight, counts)
+    return _product(x, weight, bias, counts, False)
+
+
+def packed_linear(x, weight: PackedWeight, bias=None):
+    """x [..., K] -> x W^T + bias [..., N], in x's dtype (float16 / bfloat16).
+
+    One row reads the weight at memory speed, many rows run on the matrix cores; the values of the codes enter the
+    products exactly and the scales are applied in float32.  Differentiable in x and bias (once)."""
+    bias = _check_operands(x, weight, bias)
+    if weight.experts is not None:
+        raise ValueError("a stack of experts goes through packed_expert_linear")
+    y = _run(x if x.dim() == 2 else x.reshape(-1, weight.k), weight, bias, None)
+    return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (weight.n,))
+
+
+def packed_expert_linear(x, weight: PackedWeight, counts, bias=None):
+    """x [R, K], rows sorted by expert -> [R, N] with row r times the weight (plus the bias row) of its expert.
+
+    counts: int32 or int64 [E] on x's device, the number of rows of each expert; it is never read by the host, so a
+    call can be captured and replayed with other counts.  Rows behind the last expert's come back as zeros; counts that
+    add up to more than R are cut off there.  Differentiable in x and bias (once)."""
+    bias = _check_operands(x, weight, bias)
+    if weight.experts is None:
+        raise ValueError("a single weight goes through packed_linear")
+    if x.dim() != 2:
+        raise ValueError(f"rows [R, {weight.k}] are wanted, got {tuple(x.shape)}")
+    if not isinstance(counts, torch.Tensor) or counts.dtype not in (torch.int32, torch.int64) \
+            or tuple(counts.shape) != (weight.experts,) or counts.device != x.device:
+        raise ValueError(f"counts: int32 or int64 [{weight.experts}] on {x.device} wanted")
+    if counts.dtype == torch.int64:
+        counts = counts.clamp(0, x.shape[0]).to(torch.int32)
+    return _run(x, weight, bias, counts.contiguous())
+
+
+class PackedLinear(nn.Module):
+    """A Linear whose weight is held in 4 bits: quantizes src.weight with pack_weight; the bias stays a parameter."""
+
+    def __init__(self, src: nn.Linear, wq_bits: int = 4, datatype: str = "int4", group_size=None):
+        super().__init__()
+        self.in_features, self.out_features = src.in_features, src.out_features
+        self.packed = pack_weight(src.weight.data, wq_bits, datatype, group_size)
+        for name in ("data", "params", "norm"):
+            self.register_buffer("weight_" + name, getattr(self.packed, name))
+        self.bias = None if src.bias is None else nn.Parameter(src.bias.detach().to(self.packed.device),
+                                                               requires_grad=src.bias.requires_grad)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)   # buffers may have moved: the description holds their addresses
+        p = self.packed
+        self.packed = PackedWeight(self.weight_data, self.weight_params, self.weight_norm, p.experts, p.n, p.k, p.group_size,
+                                   p.wq_bits, p.datatype)
+        return self
+
+    def forward(self, x):
+        return packed_linear(x, self.packed, self.bias)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, {self.packed}"

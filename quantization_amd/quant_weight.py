@@ -243,16 +243,29 @@ def _linears(model):
 
 
 def quant_model(model, wq_bits: Optional[int] = None, wq_datatype: Optional[str] = None,
-                wq_groupsize: Optional[int] = None, _dump_int: bool = True):
+                wq_groupsize: Optional[int] = None, _dump_int: bool = True, packed: bool = False):
     """Fake-quantize every nn.Linear weight in place, then (unless _dump_int is False) swap each Linear
     for a _LinearDump holding codes / scales / zero-points (quant_weight.py:652-706, :921-936).
     Dispatch on the datatype string follows the reference's order.
 
     The reference loops over the layers; here the Linear weights are grouped by (shape, dtype, device) and
     every group goes through one fused launch per 32 layers, once for the dequantized weights and once more
-    -- on the already dequantized weights, as the reference's _LinearDump does (:882-895) -- for the codes."""
+    -- on the already dequantized weights, as the reference's _LinearDump does (:882-895) -- for the codes.
+
+    packed: swap each Linear for a packed.PackedLinear instead, which holds the weight's codes in 4 bits and multiplies by
+    them (integers of 2 to 4 bits and the 3- and 4-bit tables; ValueError for the other formats).  The codes are those of
+    the weight itself, and the model then lives on the ROCm device; no counterpart in the reference."""
     if wq_datatype is None or wq_datatype in ("fp16", "fp32"):
         print("Not applying quantization")
+        return
+    if packed:
+        from .packed import PackedLinear, _kind_of
+        _kind_of(wq_bits, wq_datatype)
+        print(f"Packing weights in 4 bits: {wq_bits}-bit {wq_datatype}, group size: {wq_groupsize}")
+        linears = [(name, PackedLinear(m, wq_bits, wq_datatype, wq_groupsize)) for name, m in _linears(model)]
+        for name, mod in linears:   # (only once every weight has been packed: a refused one leaves the model as it was)
+            parent, attr = _find_parent(model, name)
+            setattr(parent, attr, mod)
         return
     if wq_datatype.startswith("int"):
         asym = "asym" in wq_datatype
