@@ -147,7 +147,10 @@ def prepare(case, seed):
     if own:
         from quantization_amd import packed
         s["calls"] = packed
-        s["weight"] = packed.pack_codes(s.pop("q"), s.pop("scale"), s.pop("zero"), wq_bits=4, datatype=case["format"],
+        scale, zero = s.pop("scale"), s.pop("zero")
+        if not case["group"]:   # one scale per row: without the groups' axis
+            scale, zero = scale[..., 0], None if zero is None else zero[..., 0]
+        s["weight"] = packed.pack_codes(s.pop("q"), scale, zero, wq_bits=4, datatype=case["format"],
                                         group_size=case["group"] or None)
         s["counts"] = s["counts"].to(device="cuda", dtype=torch.int32)
         s["leaves"] = [t.requires_grad_() for t in (s["x"], s["bias"]) if t is not None] if s["train"] else []
