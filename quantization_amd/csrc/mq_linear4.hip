@@ -109,6 +109,13 @@ template <int KIND> __global__ __launch_bounds__(256) void k_w4_unpack(const W4A
   }
 }
 
+// ---- rows that k_w4_gemm cannot read as they are ----------------------------------------------------
+// Rows of any stride, alignment and length -> rows of 128 rb elements, zeros behind the end.
+__global__ __launch_bounds__(256) void k_w4_pad(const W4Product p, int64_t rows, uint16_t* to) {
+  const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), k = (int64_t)blockIdx.y * 128 + (threadIdx.x & 15) * 8;
+  if (r < rows) *reinterpret_cast<u32x4*>(to + r * p.rb * 128 + k) = w4_load8(p.x + r * p.ldx, k, p.kc, p.vec);
+}
+
 // ---- the transposed operand of the gradient ----------------------------------------------------------
 // dx = dy W contracts over the weight's rows: the same codes in the same layout with the roles of rows and columns
 // exchanged.  A thread turns 8 rows x 8 columns.  Bound by its own bytes (half a byte read and written per weight).
@@ -225,7 +232,7 @@ int fill_args(const mq_w4* w, const int32_t* counts, int64_t rows, W4Args* a) {
   a->kt = (int32_t)w4_ktiles(w->k);
   a->gu = steps_of_group(w);
   a->gp = groups_padded(w);
-  a->gmagic = a->gu > 1 ? (uint32_t)((((uint64_t)1 << 32) + a->gu - 1) / a->gu) : 0;
+  a->gmagic = (uint32_t)((((uint64_t)1 << 31) + a->gu - 1) / a->gu);
   if (w->kind == W4_LUT) {
     bool ok = true;
     for (int i = 0; i < 16; ++i) a->lut.w[i / 4] |= (uint32_t)e4m3_of(w->values[i], &ok) << (8 * (i % 4));
@@ -258,7 +265,7 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
     return pl;
   }
   pl.bm = per <= 64 ? 64 : 128;
-  pl.bn = 128;
+  pl.bn = pl.bm == 64 ? 128 : W4_CFG_BN;
   p->nblocks = (p->ct * 16 + pl.bn - 1) / pl.bn;
   p->mblocks = (int32_t)row_blocks(pl.bm);
   // fewer tiles than compute units: the contraction is cut, at least 4 blocks of 128 to a piece
@@ -269,7 +276,13 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 size_t turned_bytes(const mq_w4* w) { return (size_t)w->experts * w4_ntiles(w->k) * w4_ktiles(w->n) * 1024; }
-size_t part_bytes(const W4Product& p, int64_t rows) { return p.splits > 1 ? (size_t)p.splits * rows * p.ct * 16 * 4 : 0; }
+size_t part_bytes(const W4Product& p, int64_t rows) {
+  return p.splits > 1 ? up256((size_t)p.splits * rows * p.ct * 16 * 4) : 0;
+}
+// the row sums for the zero points (k_w4_rowsum)
+size_t sums_bytes(const mq_w4* w, const W4Plan& pl, const W4Product& p, int64_t rows, bool grad) {
+  return pl.bm && !grad && w->kind == W4_U4 ? up256(((size_t)p.rb * (4 / pl.fs) * rows + pl.bm) * 4) : 0;  // (a tile reads past the last row)
+}
 
 int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
             const int32_t* counts, void* y, void* ws, size_t ws_bytes, void* stream, bool grad) {
@@ -288,18 +301,30 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   W4Product p = {};
   const W4Plan pl = plan_of(w, rows, grad, counts != nullptr, &p);
   if ((int64_t)p.nblocks * p.mblocks > (int64_t)0x7FFFFFFF) return MQ_ERR_TOO_LARGE;
-  const size_t turned = grad ? up256(turned_bytes(w)) : 0;
-  const size_t need = turned + part_bytes(p, rows);
+  p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
+  // workspace: the turned operand (gradient) or the row sums, the splits' partial sums, the padded rows
+  const size_t sums = sums_bytes(w, pl, p, rows, grad), turned = grad ? up256(turned_bytes(w)) : sums;
+  const size_t padded = pl.bm && (!p.vec || kc % 128) ? (size_t)rows * p.rb * 256 : 0;
+  const size_t need = turned + part_bytes(p, rows) + padded;
   if (need && (!ws || ws_bytes < need)) return MQ_ERR_WORKSPACE;
   if (need && (uintptr_t)ws % 16) return MQ_ERR_ALIGN;
   p.x = static_cast<const uint16_t*>(x);
   p.ldx = ldx;
-  p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
   p.b = a.data;
   p.bias = static_cast<const uint16_t*>(bias);
   p.y = static_cast<uint16_t*>(y);
   p.part = p.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(ws) + turned) : nullptr;
+  p.xs = sums ? static_cast<float*>(ws) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (padded) {
+    uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + turned + part_bytes(p, rows));
+    hipLaunchKernelGGL(k_w4_pad, dim3((unsigned)((rows + 15) / 16), p.rb), dim3(256), 0, st, p, rows, to);
+    MQ_HIP(hipGetLastError());
+    p.x = to;
+    p.ldx = (int64_t)p.rb * 128;
+    p.kc = p.ldx;
+    p.vec = 1;
+  }
   if (grad) {
     uint32_t* t = static_cast<uint32_t*>(ws);
     const dim3 grid(a.kt, p.rb, (unsigned)w->experts);
@@ -414,11 +439,12 @@ extern "C" int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream) {
   }
   return MQ_OK;
 }
-extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t counted, int32_t grad) {
+extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t aligned, int32_t counted, int32_t grad) {
   if (check_w4(w) != MQ_OK || rows < 1 || rows > kMaxRows) return 0;
   W4Product p = {};
-  plan_of(w, rows, grad != 0, counted != 0, &p);
-  return (grad ? up256(turned_bytes(w)) : 0) + part_bytes(p, rows);
+  const W4Plan pl = plan_of(w, rows, grad != 0, counted != 0, &p);
+  return (grad ? up256(turned_bytes(w)) : sums_bytes(w, pl, p, rows, false)) + part_bytes(p, rows) +
+         (pl.bm && (!aligned || p.kc % 128) ? (size_t)rows * p.rb * 256 : 0);
 }
 extern "C" int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
                           const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream) {

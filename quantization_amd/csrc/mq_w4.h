@@ -25,6 +25,7 @@ typedef _Float16 w4_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 w4_h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 w4_b2 __attribute__((ext_vector_type(2)));
 typedef __bf16 w4_b8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float w4_f2 __attribute__((ext_vector_type(2)));
 
 struct W4Lut {
@@ -96,6 +97,9 @@ struct W4F16 {  // element traits: float16
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(w4_h8, a), __builtin_bit_cast(w4_h8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(w4_h8, a), __builtin_bit_cast(w4_h8, b), c, 0, 0, 0);
+  }
   static constexpr uint32_t kOnes = 0x3C003C00u;
 };
 struct W4BF16 {  // element traits: bfloat16
@@ -117,6 +121,9 @@ struct W4BF16 {  // element traits: bfloat16
   static __device__ __forceinline__ uint16_t from_f32(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(w4_b8, a), __builtin_bit_cast(w4_b8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(w4_b8, a), __builtin_bit_cast(w4_b8, b), c, 0, 0, 0);
   }
   static constexpr uint32_t kOnes = 0x3F803F80u;
 };
@@ -161,6 +168,8 @@ template <int KIND> __device__ __forceinline__ void w4_decode_f32(uint32_t d, co
   for (int i = 0; i < 4; ++i) f[2 * i] = p[i][0], f[2 * i + 1] = p[i][1];
 }
 
+__device__ __forceinline__ f32x16 w4_zero16() { return f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
+
 // ---- the arguments that all kernels share ------------------------------------------------------------
 struct W4Args {
   const uint32_t* data;    // [E][NT][KT][64][4]
@@ -170,12 +179,13 @@ struct W4Args {
   int64_t experts, n, k, rows;
   int32_t nt, kt, gp;      // tiles along N and K, groups along the padded K
   int32_t gu;              // K-steps of 32 per group
-  uint32_t gmagic;         // group of K-step s = mulhi(s, gmagic) (gu > 1; exact for s * gu < 2^32)
+  uint32_t gmagic;         // ceil(2^31 / gu): see w4_group
   W4Lut lut;
 };
-__device__ __forceinline__ int w4_group(const W4Args& a, int step) {
-  return a.gu == 1 ? step : (int)__umulhi((uint32_t)step, a.gmagic);
-}
+// Group of K-step s: floor(s / gu) = floor((2 s + 1) / (2 gu)) as the high half of (2 s + 1) * ceil(2^32 / (2 gu)).  The
+// product is too large by (2 s + 1) * d / 2^32 with d < 2 gu, and the fraction leaves 1 / (2 gu) of room: exact for
+// (2 s + 1) * 2 gu <= 2^32, and s, gu < 2^15 (columns <= 2^20).
+__device__ __forceinline__ int w4_group(const W4Args& a, int step) { return (int)__umulhi((uint32_t)(2 * step + 1), a.gmagic); }
 
 // Row tile t -> (expert, first row, rows).  Experts without rows have no tiles; counts below zero stand for none and the
 // sum stops at `rows`, whatever the array holds, so that every row is in bounds; the rows behind the last expert's form

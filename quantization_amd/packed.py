@@ -44,7 +44,7 @@ def _bind():
         L.mq_w4_params_bytes.restype, L.mq_w4_params_bytes.argtypes = sz, [pw]
         L.mq_w4_pack.restype, L.mq_w4_pack.argtypes = ctypes.c_int, [pw, vp, vp, vp, vp]
         L.mq_w4_unpack.restype, L.mq_w4_unpack.argtypes = ctypes.c_int, [pw, vp, vp]
-        L.mq_linear4_workspace_bytes.restype, L.mq_linear4_workspace_bytes.argtypes = sz, [pw, i64, i32, i32]
+        L.mq_linear4_workspace_bytes.restype, L.mq_linear4_workspace_bytes.argtypes = sz, [pw, i64, i32, i32, i32]
         L.mq_linear4.restype, L.mq_linear4.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, vp, sz, vp]
         L.mq_linear4_grad.restype, L.mq_linear4_grad.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, sz, vp]
         L.mq_bias_grad_workspace_bytes.restype, L.mq_bias_grad_workspace_bytes.argtypes = sz, [i64, i64, i64]
@@ -265,7 +265,8 @@ def _product(t, weight, bias, counts, grad):
     t, ld = _rows_of(t)
     cp = None if counts is None else counts.data_ptr()
     with torch.cuda.device(t.device):
-        need = L.mq_linear4_workspace_bytes(weight._ref, rows, counts is not None, grad)
+        aligned = t.data_ptr() % 16 == 0 and (ld % 8 == 0 or rows == 1)
+        need = L.mq_linear4_workspace_bytes(weight._ref, rows, aligned, counts is not None, grad)
         # of this call alone: a captured graph keeps it in its own pool, and calls on other streams have their own
         ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
         wp = None if ws is None else ws.data_ptr()

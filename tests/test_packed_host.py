@@ -59,7 +59,7 @@ def test_library_refuses_before_any_launch():
     bad = _c(kind=packed.TABLE)
     bad.values[1] = 17.5                                        # not an e4m3 number
     assert call(bad) == _lib.ERR_UNSUPPORTED
-    need = L.mq_linear4_workspace_bytes(ref(_c()), 4, 0, 1)     # the gradient's turned operand
+    need = L.mq_linear4_workspace_bytes(ref(_c()), 4, 1, 0, 1)     # the gradient's turned operand
     assert need >= 16 * 1024
     assert L.mq_linear4_grad(ref(_c()), 4096, _lib.F16, 4, 64, None, 4096, None, 0, None) == _lib.ERR_WORKSPACE
     assert L.mq_linear4_grad(ref(_c()), 4096, _lib.F16, 4, 64, None, 4096, 4096, need - 1, None) == _lib.ERR_WORKSPACE
