@@ -118,25 +118,111 @@ __global__ __launch_bounds__(256) void k_w4_pad(const W4Product p, int64_t rows,
 
 // ---- the transposed operand of the gradient ----------------------------------------------------------
 // dx = dy W contracts over the weight's rows: the same codes in the same layout with the roles of rows and columns
-// exchanged.  A thread turns 8 rows x 8 columns.  Bound by its own bytes (half a byte read and written per weight).
-template <int KIND>
-__global__ __launch_bounds__(256) void k_w4_turn(const W4Args a, uint32_t* out, int32_t ct, int32_t rb) {
-  const int t = threadIdx.x, c = t & 15, nb = t >> 4;
+// exchanged.  A wave turns 128 rows x 128 columns, a thread 8 rows x 32 columns: it
+// reads four dwords of each row at once (8 x 16 contiguous bytes) and turns four blocks of 8 x 8 nibbles in registers, by
+// exchanging nibbles, bytes and halves between pairs of dwords (32 instructions a block).  The turned dwords go through
+// LDS, so that whole tiles are stored.  Bound by its bytes: half a byte read and written per weight.
+// It also writes the scales (and zero points) along the contraction, in the form that W4Scales loads.
+struct TurnArgs {
+  uint32_t* out;  // [E][ct][rb][64][4]
+  void* ts;       // [E][GP][128 rb]
+  void* tz;
+  int32_t ct, rb, half;
+};
+// Nibble r of b[c] = nibble c of a[r].
+__device__ __forceinline__ void w4_turn8(uint32_t* a) {
+#pragma unroll
+  for (int r = 0; r < 8; r += 2) {
+    const uint32_t x = a[r], y = a[r + 1];
+    a[r] = (x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u);
+    a[r + 1] = ((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = (i & 1) + (i >> 1) * 4;
+    const uint32_t x = a[r], y = a[r + 2];
+    a[r] = __builtin_amdgcn_perm(y, x, 0x06020400u);
+    a[r + 2] = __builtin_amdgcn_perm(y, x, 0x07030501u);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t x = a[r], y = a[r + 4];
+    a[r] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+    a[r + 4] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+  }
+}
+template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args a, const TurnArgs t) {
+  __shared__ u32x4 lds[512];
+  const int lane = threadIdx.x, kq = lane & 3, nb = lane >> 2;
   const int64_t e = blockIdx.z;
   if (a.counts && a.counts[e] <= 0) return;
   const int64_t nt = (int64_t)blockIdx.y * 8 + (nb >> 1);
-  uint32_t d[8];
+  u32x4 in[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    d[i] = nt < a.nt ? a.data[((e * a.nt + nt) * a.kt + blockIdx.x) * 256 + ((c & 3) * 16 + (nb & 1) * 8 + i) * 4 + (c >> 2)] : 0u;
+  for (int i = 0; i < 8; ++i) {
+    in[i] = {0, 0, 0, 0};
+    if (nt < a.nt)
+      in[i] = *reinterpret_cast<const u32x4*>(a.data + ((e * a.nt + nt) * a.kt + blockIdx.x) * 256 + (kq * 16 + (nb & 1) * 8 + i) * 4);
+  }
+  uint32_t* flat = reinterpret_cast<uint32_t*>(lds);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    uint32_t o = 0;
+  for (int j = 0; j < 4; ++j) {
+    // the code at slot i of a dword stands in nibble at(i); rows and columns are both taken in the order of the nibbles
+    uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o |= w4_put<KIND>(w4_get<KIND>(d[i], q), i);
-    const int k = c * 8 + q;  // c = octet index: 4 * j + kq = (32 j + 8 kq) / 8
-    const int64_t tile = (int64_t)blockIdx.x * 8 + (k >> 4);
-    if (tile < ct) out[((e * ct + tile) * rb + blockIdx.y) * 256 + ((nb & 3) * 16 + (k & 15)) * 4 + (nb >> 2)] = o;
+    for (int i = 0; i < 8; ++i) {
+      const int at = KIND == W4_FP4 ? i : i < 4 ? 2 * i : 2 * (i - 4) + 1;
+      uint32_t d = in[i][j];
+      if constexpr (KIND == W4_S4 || KIND == W4_LUT) d = (d & 0x77777777u) | (__builtin_amdgcn_alignbit(d, d, 4) & 0x88888888u);
+      b[at] = d;
+    }
+    w4_turn8(b);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int at = KIND == W4_FP4 ? q : q < 4 ? 2 * q : 2 * (q - 4) + 1;
+      uint32_t d = b[at];
+      if constexpr (KIND == W4_S4 || KIND == W4_LUT) d = (d & 0x77777777u) | (__builtin_amdgcn_alignbit(d, d, 28) & 0x88888888u);
+      const int k = j * 32 + kq * 8 + q;  // column in the block; n = 8 nb + i: dword nb / 4 of lane 16 (nb % 4) + k % 16
+      const int pos = (k >> 4) * 256 + ((nb & 3) * 16 + (k & 15)) * 4 + (nb >> 2);
+      flat[pos ^ (((pos >> 6 & 3) | (pos >> 8 & 1) << 2) << 2)] = d;  // (spread over the banks)
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t tile = (int64_t)blockIdx.x * 8 + i;
+    if (tile < t.ct) {
+      const int pos = i * 64 + lane;
+      reinterpret_cast<u32x4*>(t.out)[((e * t.ct + tile) * t.rb + blockIdx.y) * 64 + lane] = lds[pos ^ ((pos >> 4 & 3) | (pos >> 6 & 1) << 2)];
+    }
+  }
+  // scales of the groups that begin in this block of columns
+  const float up = t.half ? a.norm[e] : w4_f32_scale<KIND>();
+  for (int j = 0; j < 4; ++j) {
+    const int step = blockIdx.x * 4 + j, grp = w4_group(a, step);
+    if (grp * a.gu != step || grp >= a.gp) continue;
+    for (int i = lane; i < 128; i += 64) {
+      const int64_t n = (int64_t)blockIdx.y * 128 + i, tile = n >> 4;
+      float s = 0, z = 0;
+      if (tile < a.nt) {
+        const int64_t at = ((e * a.nt + tile) * a.gp + grp) * 16 + (n & 15);
+        if constexpr (KIND == W4_U4) {
+          const uint32_t v = static_cast<const uint32_t*>(a.params)[at];
+          s = (float)h_from_bits(v);
+          z = (float)h_from_bits(v >> 16);
+        } else {
+          s = (float)h_from_bits(static_cast<const uint16_t*>(a.params)[at]);
+        }
+      }
+      const int64_t to = (e * a.gp + grp) * t.rb * 128 + n;
+      if (t.half) {
+        static_cast<uint16_t*>(t.ts)[to] = W4F16::from_f32(s * up);
+        if constexpr (KIND == W4_U4) static_cast<uint16_t*>(t.tz)[to] = W4F16::from_f32(z);
+      } else {
+        static_cast<float*>(t.ts)[to] = s * up;
+        if constexpr (KIND == W4_U4) static_cast<float*>(t.tz)[to] = s * z;  // exact: 11 x 11 bits
+      }
+    }
   }
 }
 
@@ -265,7 +351,7 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
     return pl;
   }
   pl.bm = per <= 64 ? 64 : 128;
-  pl.bn = pl.bm == 64 ? 128 : W4_CFG_BN;
+  pl.bn = grad && pl.bm == 128 ? 256 : 128;
   p->nblocks = (p->ct * 16 + pl.bn - 1) / pl.bn;
   p->mblocks = (int32_t)row_blocks(pl.bm);
   // fewer tiles than compute units: the contraction is cut, at least 4 blocks of 128 to a piece
@@ -275,7 +361,11 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
-size_t turned_bytes(const mq_w4* w) { return (size_t)w->experts * w4_ntiles(w->k) * w4_ktiles(w->n) * 1024; }
+size_t turned_bytes(const mq_w4* w) { return up256((size_t)w->experts * w4_ntiles(w->k) * w4_ktiles(w->n) * 1024); }
+size_t turned_params_bytes(const mq_w4* w) {  // of one of the two arrays, float32 at most
+  return up256((size_t)w->experts * groups_padded(w) * w4_ktiles(w->n) * 128 * 4);
+}
+size_t turn_bytes(const mq_w4* w) { return turned_bytes(w) + 2 * turned_params_bytes(w); }
 size_t part_bytes(const W4Product& p, int64_t rows) {
   return p.splits > 1 ? up256((size_t)p.splits * rows * p.ct * 16 * 4) : 0;
 }
@@ -303,7 +393,7 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   if ((int64_t)p.nblocks * p.mblocks > (int64_t)0x7FFFFFFF) return MQ_ERR_TOO_LARGE;
   p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
   // workspace: the turned operand (gradient) or the row sums, the splits' partial sums, the padded rows
-  const size_t sums = sums_bytes(w, pl, p, rows, grad), turned = grad ? up256(turned_bytes(w)) : sums;
+  const size_t sums = sums_bytes(w, pl, p, rows, grad), turned = grad ? turn_bytes(w) : sums;
   const size_t padded = pl.bm && (!p.vec || kc % 128) ? (size_t)rows * p.rb * 256 : 0;
   const size_t need = turned + part_bytes(p, rows) + padded;
   if (need && (!ws || ws_bytes < need)) return MQ_ERR_WORKSPACE;
@@ -326,15 +416,20 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
     p.vec = 1;
   }
   if (grad) {
-    uint32_t* t = static_cast<uint32_t*>(ws);
+    char* at = static_cast<char*>(ws);
+    const TurnArgs t = {reinterpret_cast<uint32_t*>(at), at + turned_bytes(w), at + turned_bytes(w) + turned_params_bytes(w),
+                        p.ct, p.rb, dtype == MQ_F16};
     const dim3 grid(a.kt, p.rb, (unsigned)w->experts);
     switch (w->kind) {
-      case W4_U4: hipLaunchKernelGGL((k_w4_turn<W4_U4>), grid, dim3(256), 0, st, a, t, p.ct, p.rb); break;
-      case W4_FP4: hipLaunchKernelGGL((k_w4_turn<W4_FP4>), grid, dim3(256), 0, st, a, t, p.ct, p.rb); break;
-      default: hipLaunchKernelGGL((k_w4_turn<W4_S4>), grid, dim3(256), 0, st, a, t, p.ct, p.rb); break;  // LUT: the same bits
+      case W4_U4: hipLaunchKernelGGL((k_w4_turn<W4_U4>), grid, dim3(64), 0, st, a, t); break;
+      case W4_S4: hipLaunchKernelGGL((k_w4_turn<W4_S4>), grid, dim3(64), 0, st, a, t); break;
+      case W4_LUT: hipLaunchKernelGGL((k_w4_turn<W4_LUT>), grid, dim3(64), 0, st, a, t); break;
+      default: hipLaunchKernelGGL((k_w4_turn<W4_FP4>), grid, dim3(64), 0, st, a, t); break;
     }
     MQ_HIP(hipGetLastError());
-    p.b = t;
+    p.b = t.out;
+    p.ts = t.ts;
+    p.tz = t.tz;
   }
   const bool h = dtype == MQ_F16;
   hipError_t e;
@@ -443,7 +538,7 @@ extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32
   if (check_w4(w) != MQ_OK || rows < 1 || rows > kMaxRows) return 0;
   W4Product p = {};
   const W4Plan pl = plan_of(w, rows, grad != 0, counted != 0, &p);
-  return (grad ? up256(turned_bytes(w)) : sums_bytes(w, pl, p, rows, false)) + part_bytes(p, rows) +
+  return (grad ? turn_bytes(w) : sums_bytes(w, pl, p, rows, false)) + part_bytes(p, rows) +
          (pl.bm && (!aligned || p.kc % 128) ? (size_t)rows * p.rb * 256 : 0);
 }
 extern "C" int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,

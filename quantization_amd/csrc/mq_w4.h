@@ -78,6 +78,7 @@ template <int KIND> __device__ __forceinline__ void w4_bytes(uint32_t d, const W
 template <int KIND> constexpr float w4_byte_scale() { return KIND == W4_U4 || KIND == W4_S4 ? 512.0f : 1.0f; }
 
 struct W4F16 {  // element traits: float16
+  static constexpr bool kHalf = true;
   typedef _Float16 elem;
   typedef w4_h8 vec8;
   template <bool HI> static __device__ __forceinline__ uint32_t from_fp8(uint32_t v, float s) {
@@ -103,6 +104,7 @@ struct W4F16 {  // element traits: float16
   static constexpr uint32_t kOnes = 0x3C003C00u;
 };
 struct W4BF16 {  // element traits: bfloat16
+  static constexpr bool kHalf = false;
   typedef __bf16 elem;
   typedef w4_b8 vec8;
   template <bool HI> static __device__ __forceinline__ uint32_t from_fp8(uint32_t v, float s) {

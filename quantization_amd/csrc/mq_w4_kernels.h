@@ -3,10 +3,6 @@
 //
 #pragma once
 #include "mq_w4.h"
-#ifndef W4_CFG
-#define W4_CFG 2, 2, 2, 2
-#define W4_CFG_BN 128
-#endif
 
 struct W4Product {
   const uint16_t* x;     // [rows][ldx], contraction index contiguous
@@ -15,6 +11,8 @@ struct W4Product {
   uint16_t* y;           // [rows][nc]
   float* part;           // [splits][rows][16 * ct] partial sums, NULL when splits == 1
   float* xs;             // sums of x per window and row (k_w4_rowsum), for zero points in k_w4_gemm
+  const void* ts;        // gradient: scales along the contraction, k_w4_turn's [E][GP][128 rb]
+  const void* tz;        // ... and zero points (float16) or scale * zero (bfloat16)
   int64_t ldx, kc, nc;   // contraction length, output columns
   int32_t ct, rb;        // 16-column tiles of the output, 128-blocks of the contraction
   int32_t vec;           // rows of x are 16-byte aligned and kc % 8 == 0
@@ -190,6 +188,47 @@ __global__ __launch_bounds__(512) void k_w4_rows(const W4Args a, const W4Product
   }
 }
 
+// ---- the gradient's scaled weights ---------------------------------------------------------------------
+// Eight weights of one column, scale * (q - zero) rounded once to T.  float16: the integer difference is exact, the
+// product rounds (scales are held times the expert's norm, a power of two); bfloat16: one float32 fma, then the rounding.
+template <class T, int KIND> struct W4Scales;
+template <int KIND> struct W4Scales<W4F16, KIND> {
+  u32x4 s, z;
+  __device__ __forceinline__ void load(const W4Product& p, int64_t at) {
+    s = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.ts) + at);
+    if constexpr (KIND == W4_U4) z = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.tz) + at);
+  }
+  __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
+    u32x4 v = w4_decode<W4F16, KIND>(d, lut);
+    // (whole vectors: the compiler takes a bit cast of one element of a vector for one of its first element)
+    w4_h8 q = __builtin_bit_cast(w4_h8, v);
+    if constexpr (KIND == W4_U4) q = q - __builtin_bit_cast(w4_h8, z);
+    return __builtin_bit_cast(u32x4, q * __builtin_bit_cast(w4_h8, s));
+  }
+};
+template <int KIND> struct W4Scales<W4BF16, KIND> {
+  f32x4 s[2], z[2];
+  __device__ __forceinline__ void load(const W4Product& p, int64_t at) {
+    const f32x4* from = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.ts) + at);
+    s[0] = from[0], s[1] = from[1];
+    if constexpr (KIND == W4_U4) {
+      const f32x4* zero = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.tz) + at);
+      z[0] = zero[0], z[1] = zero[1];
+    }
+  }
+  __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
+    float f[8];
+    w4_decode_f32<KIND>(d, lut, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      f[i] = KIND == W4_U4 ? __builtin_fmaf(f[i], s[i / 4][i % 4], -z[i / 4][i % 4]) : f[i] * s[i / 4][i % 4];
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = W4BF16::pack(f[2 * i], f[2 * i + 1]);
+    return v;
+  }
+};
+
 // ---- many rows -------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves owns 32 MT WM rows and 32 NT WN columns, in tiles of v_mfma_f32_32x32x16 (which leaves six
 // vector instructions per matrix instruction free; two 16x16x32 leave four).  Here the activations are the A operand, so
@@ -206,7 +245,7 @@ typedef __attribute__((address_space(1))) const void w4_global_t;
 typedef __attribute__((address_space(3))) void w4_lds_t;
 
 template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int FS>
-__global__ __launch_bounds__(64 * WM * WN, MT * NT > 4 ? 1 : 2) void k_w4_gemm(const W4Args a, const W4Product p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, const W4Product p) {
   constexpr int BM = 32 * MT * WM, NW = WM * WN, CH = BM / 4 / NW;  // 1 KiB pieces (4 rows) per wave
   static_assert(BM / 4 % NW == 0, "the rows of a block are dealt evenly");
   __shared__ u32x4 lds[2][BM * 16];
@@ -246,6 +285,12 @@ __global__ __launch_bounds__(64 * WM * WN, MT * NT > 4 ? 1 : 2) void k_w4_gemm(c
       xp[c] = p.x + (row0 + (r < rows ? r : rows - 1)) * p.ldx + (((lane & 15) ^ (r & 15)) * 8);
     }
     const int kb0 = (int)((int64_t)p.rb * blockIdx.y / p.splits), kb1 = (int)((int64_t)p.rb * (blockIdx.y + 1) / p.splits);
+    int64_t st0[NT];  // gradient: this lane's first scale under column tile n
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int64_t c = tile0 + n, last = (p.ct - 1) >> 1;
+      st0[n] = ((int64_t)expert * a.gp + w4_group(a, (int)(c < last ? c : last))) * p.rb * 128 + half * 8;
+    }
     u32x4 bn[NT][2];
     auto fetch = [&](int kb, int buf) {
 #pragma unroll
@@ -314,52 +359,17 @@ __global__ __launch_bounds__(64 * WM * WN, MT * NT > 4 ? 1 : 2) void k_w4_gemm(c
         }
       } else {
         constexpr int SETS = FS == 1 ? NT : 1;  // groups under a wave's 32 NT columns
-        const float up = a.norm[expert];
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
-          float s[SETS][8], sz[SETS][8];
-          const int64_t n0 = (int64_t)kb * 128 + st * 16;
-          const int64_t nt = (int64_t)expert * a.nt + (n0 / 16 < a.nt ? n0 / 16 : a.nt - 1);
+          W4Scales<T, KIND> sc[SETS];
 #pragma unroll
-          for (int g = 0; g < SETS; ++g) {
-            const int64_t c = tile0 + g, last = (p.ct - 1) >> 1;
-            const int64_t at = (nt * a.gp + w4_group(a, (int)(c < last ? c : last))) * 16 + half * 8;
-            if constexpr (KIND == W4_U4) {
-              const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const uint32_t*>(a.params) + at);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const u32x4 v = q[h];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  s[g][4 * h + i] = (float)h_from_bits(v[i]) * up;
-                  sz[g][4 * h + i] = s[g][4 * h + i] * (float)h_from_bits(v[i] >> 16);
-                }
-              }
-            } else {
-              const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.params) + at);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                s[g][2 * i] = (float)h_from_bits(v[i]) * up;
-                s[g][2 * i + 1] = (float)h_from_bits(v[i] >> 16) * up;
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[g][i] *= w4_f32_scale<KIND>();
-          }
+          for (int g = 0; g < SETS; ++g) sc[g].load(p, st0[g] + kb * 128 + st * 16);
           u32x4 xv[MT];
 #pragma unroll
           for (int m = 0; m < MT; ++m) xv[m] = xb[m * 512 + ((2 * st) ^ turn)];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float f[8];
-            w4_decode_f32<KIND>(bv[n][st & 1][st >> 1], a.lut, f);
-            const int g = FS == 1 ? n : 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              f[i] = KIND == W4_U4 ? __builtin_fmaf(f[i], s[g][i], -sz[g][i]) : f[i] * s[g][i];
-            u32x4 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = T::pack(f[2 * i], f[2 * i + 1]);
+            const u32x4 v = sc[FS == 1 ? n : 0].scaled(bv[n][st & 1][st >> 1], a.lut);
 #pragma unroll
             for (int m = 0; m < MT; ++m) acc[m][n] = T::mfma32(xv[m], v, acc[m][n]);
           }
@@ -368,7 +378,7 @@ __global__ __launch_bounds__(64 * WM * WN, MT * NT > 4 ? 1 : 2) void k_w4_gemm(c
       __syncthreads();
     }
     if constexpr (GRAD) {
-      const float down = 1.0f / a.norm[expert];  // a power of two
+      const float down = T::kHalf ? 1.0f / a.norm[expert] : 1.0f;  // (float16 weights are held times norm, a power of two)
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -487,10 +497,11 @@ hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool
     else w4_rows_go<T, KIND, 2, 4>(a, p, pl, st);
   } else if (grad) {
     if (pl.bm == 64) w4_gemm_go<T, KIND, true, 1, 2, 2, 2>(a, p, pl, st);
-    else w4_gemm_go<T, KIND, true, W4_CFG>(a, p, pl, st);
+    else if (pl.bn == 256) w4_gemm_go<T, KIND, true, 4, 2, 1, 4>(a, p, pl, st);
+    else w4_gemm_go<T, KIND, true, 2, 2, 2, 2>(a, p, pl, st);
   } else {
     if (pl.bm == 64) w4_gemm_go<T, KIND, false, 1, 2, 2, 2>(a, p, pl, st);
-    else w4_gemm_go<T, KIND, false, W4_CFG>(a, p, pl, st);
+    else w4_gemm_go<T, KIND, false, 2, 2, 2, 2>(a, p, pl, st);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.part) return e;
