@@ -660,7 +660,8 @@ int mq_w4_pack(const mq_w4* w, const void* codes, const void* scale, const void*
 /* deq float16 [experts][n][k] = h(h(q - zero) * scale): the bits that the quantizers' own deq output has. */
 int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream);
 
-/* May be 0.  aligned: every row of x (dy) starts on a multiple of 16 bytes; other rows may have to be copied first.
+/* May be 0.  aligned: every row of x (dy) starts on a multiple of 16 bytes and the next one at most 2^25 elements on;
+ * other rows are copied first.
  * counted: counts will be given; grad: for mq_linear4_grad. */
 size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t aligned, int32_t counted, int32_t grad);
 /* x [rows][ldx] (ldx elements from row to row, 0 = the same row again), y [rows][n] contiguous, 16-byte aligned. */

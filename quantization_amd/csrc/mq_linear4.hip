@@ -109,7 +109,7 @@ template <int KIND> __global__ __launch_bounds__(256) void k_w4_unpack(const W4A
   }
 }
 
-// ---- rows that k_w4_gemm cannot read as they are ----------------------------------------------------
+// ---- rows that the products cannot read as they are -------------------------------------------------
 // Rows of any stride, alignment and length -> rows of 128 rb elements, zeros behind the end.
 __global__ __launch_bounds__(256) void k_w4_pad(const W4Product p, int64_t rows, uint16_t* to) {
   const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), k = (int64_t)blockIdx.y * 128 + (threadIdx.x & 15) * 8;
@@ -272,7 +272,8 @@ template <class T> __global__ __launch_bounds__(256) void k_w4_bias_join(const B
 // ---- host side -----------------------------------------------------------------------------------------
 namespace {
 
-constexpr int64_t kMaxK = 1 << 20, kMaxN = 1 << 22, kMaxExperts = 4096, kMaxRows = (int64_t)1 << 30;
+constexpr int64_t kMaxK = 1 << 20, kMaxN = 1 << 22, kMaxExperts = 4096, kMaxRows = (int64_t)1 << 29;
+constexpr int64_t kMaxStride = 1 << 25;  // elements between rows that the kernels address in 32 bits
 
 uint8_t e4m3_of(float v, bool* ok) {  // exact, or *ok = false
   for (int b = 0; b < 256; ++b) {
@@ -327,6 +328,7 @@ int fill_args(const mq_w4* w, const int32_t* counts, int64_t rows, W4Args* a) {
   return MQ_OK;
 }
 
+// Which kernel and launch shape.  Everything goes by sizes; times are microseconds per call in a graph, launch included.
 W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product* p) {
   W4Plan pl = {};
   const int32_t gu = steps_of_group(w);
@@ -337,26 +339,47 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
   p->rb = (int32_t)w4_ktiles(p->kc);
   p->splits = 1;
   const int64_t per = counted ? (rows + w->experts - 1) / w->experts : rows;  // rows of an expert, on average
+  const int64_t busy = counted ? (rows < w->experts ? rows : w->experts) : 1;  // experts that have rows, at most
   auto row_blocks = [&](int bm) {
     if (!counted) return (rows + bm - 1) / bm;
     return rows / bm + (rows < w->experts + 1 ? rows : w->experts + 1);  // every expert may end inside a tile
   };
   if (!grad && per <= 32) {
+    // Up to 32 rows k_w4_rows reads the weight at most twice; from 33 on the tiles of k_w4_gemm share it (4096 x 4096:
+    // 32 rows 10.5 against 13.5, 64 rows 17 against 15).
     pl.mt = per <= 16 ? 1 : 2;
-    pl.nt = per > 4 && p->ct >= 2048 ? 4 : 1;
-    p->nblocks = (p->ct + pl.nt - 1) / pl.nt;
     p->mblocks = (int32_t)row_blocks(16 * pl.mt);
-    pl.waves = 8;
-    while (pl.waves > 1 && pl.waves > p->rb) pl.waves /= 2;
+    const int64_t tiles = p->ct * busy;  // 16-column tiles that have rows
+    // Four column tiles to a workgroup read x a quarter as often, if enough workgroups are left (14336 x 4096, one row:
+    // 11.9, 11.0, 9.5 with one, two, four; 4096 x 4096: 4.7, 5.2, 6.8).
+    pl.nt = tiles >= 800 ? 4 : tiles >= 400 ? 2 : 1;
+    if (pl.nt < 4 && per > 4 && p->rb >= 64 && !counted) {
+      // many rows over a long contraction: reading x costs more than a second launch that joins pieces of the
+      // contraction (4096 x 14336, 16 rows: 18.0 against 14.6; one row: 11.6 against 12.8)
+      pl.nt = 4;
+      while (p->splits < 8 && tiles * p->splits < 800 && p->rb >= 16 * p->splits) p->splits *= 2;
+    }
+    p->nblocks = (p->ct + pl.nt - 1) / pl.nt;
+    const int64_t blocks = p->nblocks * busy * p->splits;
+    // waves share a workgroup's contraction: more of them only where there are few workgroups (32000 x 4096: 15.8 with
+    // four, 16.9 with eight; 14336 x 4096: 10.3 and 9.5)
+    pl.waves = blocks >= 384 ? 4 : pl.nt == 1 && pl.mt == 1 && p->rb >= 64 ? 16 : 8;
+    while (pl.waves > 1 && pl.waves * p->splits > p->rb) pl.waves /= 2;
     return pl;
   }
-  pl.bm = per <= 64 ? 64 : 128;
-  pl.bn = grad && pl.bm == 128 ? 256 : 128;
+  // Tiles of 128 rows where they occupy most compute units, 64 elsewhere (5632 x 2048, 256 rows: 24.7 against 17.6;
+  // 14336 x 4096, 256 rows: 47 against 51).  The gradient's 128 x 256 decodes half as often per product, which is what
+  // bounds it (4096 x 4096, 4096 rows: 162 against 235 with 128 x 128).
+  const int bn = grad ? 256 : 128;
+  pl.bm = (per + 127) / 128 * busy * ((p->ct * 16 + bn - 1) / bn) < (grad ? 64 : 192) ? 64 : 128;
+  pl.bn = pl.bm == 64 ? 128 : bn;
   p->nblocks = (p->ct * 16 + pl.bn - 1) / pl.bn;
   p->mblocks = (int32_t)row_blocks(pl.bm);
-  // fewer tiles than compute units: the contraction is cut, at least 4 blocks of 128 to a piece
-  const int64_t tiles = (int64_t)p->nblocks * ((rows + pl.bm - 1) / pl.bm);
-  while (p->splits < 8 && tiles * p->splits < 256 && p->rb >= 8 * p->splits) p->splits *= 2;
+  // Few tiles: the contraction is cut and the pieces joined, at least 4 blocks of 128 to a piece.  The gradient's tiles
+  // take a wave per SIMD each and want two (14336 x 4096, 2048 rows, 256 tiles: 368 against 282).
+  const int64_t tiles = (per + pl.bm - 1) / pl.bm * busy * p->nblocks;
+  const int most = grad && pl.bm == 128 ? 4 : 8;
+  while (p->splits < most && tiles * p->splits <= (grad ? 256 : 128) && p->rb >= 8 * p->splits) p->splits *= 2;
   return pl;
 }
 
@@ -394,7 +417,7 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
   // workspace: the turned operand (gradient) or the row sums, the splits' partial sums, the padded rows
   const size_t sums = sums_bytes(w, pl, p, rows, grad), turned = grad ? turn_bytes(w) : sums;
-  const size_t padded = pl.bm && (!p.vec || kc % 128) ? (size_t)rows * p.rb * 256 : 0;
+  const size_t padded = !p.vec || kc % 128 || (ldx > kMaxStride && rows > 1) ? (size_t)rows * p.rb * 256 : 0;
   const size_t need = turned + part_bytes(p, rows) + padded;
   if (need && (!ws || ws_bytes < need)) return MQ_ERR_WORKSPACE;
   if (need && (uintptr_t)ws % 16) return MQ_ERR_ALIGN;
@@ -539,7 +562,7 @@ extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32
   W4Product p = {};
   const W4Plan pl = plan_of(w, rows, grad != 0, counted != 0, &p);
   return (grad ? turn_bytes(w) : sums_bytes(w, pl, p, rows, false)) + part_bytes(p, rows) +
-         (pl.bm && (!aligned || p.kc % 128) ? (size_t)rows * p.rb * 256 : 0);
+         (!aligned || p.kc % 128 ? (size_t)rows * p.rb * 256 : 0);
 }
 extern "C" int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
                           const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream) {

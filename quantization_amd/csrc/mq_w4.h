@@ -189,52 +189,62 @@ struct W4Args {
 // (2 s + 1) * 2 gu <= 2^32, and s, gu < 2^15 (columns <= 2^20).
 __device__ __forceinline__ int w4_group(const W4Args& a, int step) { return (int)__umulhi((uint32_t)(2 * step + 1), a.gmagic); }
 
+// Inclusive sum over the lanes of a wave, cut off at `top` (0 <= v <= top < 2^30), in the vector unit's own lane moves.
+__device__ __forceinline__ uint32_t w4_scan(uint32_t v, uint32_t top) {
+#define MQ_W4_SCAN_STEP(CTRL, ROWS)                                                             \
+  {                                                                                             \
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); \
+    v = v + o < top ? v + o : top;                                                              \
+  }
+  MQ_W4_SCAN_STEP(0x111, 0xF)  // one lane up within rows of 16, then two, four, eight
+  MQ_W4_SCAN_STEP(0x112, 0xF)
+  MQ_W4_SCAN_STEP(0x114, 0xF)
+  MQ_W4_SCAN_STEP(0x118, 0xF)
+  MQ_W4_SCAN_STEP(0x142, 0xA)  // lane 15 of a row to the next row (rows 1 and 3)
+  MQ_W4_SCAN_STEP(0x143, 0xC)  // lane 31 to the upper half
+#undef MQ_W4_SCAN_STEP
+  return v;
+}
+
 // Row tile t -> (expert, first row, rows).  Experts without rows have no tiles; counts below zero stand for none and the
 // sum stops at `rows`, whatever the array holds, so that every row is in bounds; the rows behind the last expert's form
 // tiles of their own, expert = -1.  -> false when there is no tile t.  Called by whole waves.
-__device__ __forceinline__ bool w4_find_tile(const W4Args& a, int bm, int64_t t, int& expert, int64_t& row0, int& rows) {
+__device__ __forceinline__ bool w4_find_tile(const W4Args& a, int bm, int t, int& expert, int64_t& row0, int& rows) {
   if (!a.counts) {
-    row0 = t * bm;
+    row0 = (int64_t)t * bm;
     if (row0 >= a.rows) return false;
     expert = 0;
     rows = (int)(a.rows - row0 < bm ? a.rows - row0 : bm);
     return true;
   }
   const int lane = threadIdx.x & 63;
-  int64_t row_base = 0, tile_base = 0;
-  for (int64_t e0 = 0; e0 <= a.experts; e0 += 64) {  // entry `experts` is what is left
-    const int64_t e = e0 + lane;
-    int64_t c = 0;
-    if (e < a.experts) c = a.counts[e] > 0 ? a.counts[e] : 0;
-    if (e == a.experts) c = a.rows;
-    int64_t end = row_base + c;
-    int64_t s = c;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t o = __shfl_up(s, d);
-      if (lane >= d) s += o;
+  const uint32_t all = (uint32_t)a.rows;
+  uint32_t row_base = 0, tile_base = 0;
+  for (int e0 = 0; e0 <= (int)a.experts; e0 += 64) {  // entry `experts` is what is left
+    const int e = e0 + lane;
+    uint32_t c = 0;
+    if (e < (int)a.experts) {
+      const int32_t v = a.counts[e];
+      c = v > 0 ? ((uint32_t)v < all ? (uint32_t)v : all) : 0u;
     }
-    end = row_base + s < a.rows ? row_base + s : a.rows;
-    const int64_t start = row_base + s - c < a.rows ? row_base + s - c : a.rows;
-    const int64_t tiles = (end - start + bm - 1) / bm;
-    int64_t ts = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t o = __shfl_up(ts, d);
-      if (lane >= d) ts += o;
-    }
-    const bool mine = t >= tile_base + ts - tiles && t < tile_base + ts;
-    const uint64_t who = __ballot(mine);
+    if (e == (int)a.experts) c = all;
+    const uint32_t up = w4_scan(c, all);
+    const uint32_t end = row_base + up < all ? row_base + up : all;
+    const uint32_t before = (uint32_t)__shfl_up((int)end, 1), start = lane ? before : row_base;
+    const uint32_t tiles = (end - start + bm - 1) / (uint32_t)bm;
+    const uint32_t last = tile_base + w4_scan(tiles, 0x7FFFFFFFu);
+    const uint64_t who = __ballot((uint32_t)t < last);  // the first lane whose tiles reach beyond t
     if (who) {
       const int src = __builtin_ctzll(who);
-      const int64_t st = __shfl(start, src), en = __shfl(end, src), first = __shfl(tile_base + ts - tiles, src);
-      row0 = st + (t - first) * bm;
-      rows = (int)(en - row0 < bm ? en - row0 : bm);
-      expert = e0 + src < a.experts ? (int)(e0 + src) : -1;
+      const uint32_t st = (uint32_t)__builtin_amdgcn_readlane((int)start, src), en = (uint32_t)__builtin_amdgcn_readlane((int)end, src);
+      const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)(last - tiles), src);
+      row0 = st + ((uint32_t)t - first) * bm;
+      rows = (int)(en - (uint32_t)row0 < (uint32_t)bm ? en - (uint32_t)row0 : (uint32_t)bm);
+      expert = e0 + src < (int)a.experts ? e0 + src : -1;
       return true;
     }
-    row_base = __shfl(end, 63);
-    tile_base += __shfl(ts, 63);
+    row_base = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+    tile_base = (uint32_t)__builtin_amdgcn_readlane((int)last, 63);
   }
   return false;
 }

@@ -34,26 +34,6 @@ __device__ __forceinline__ u32x4 w4_load8(const uint16_t* row, int64_t k, int64_
   return v;
 }
 
-// Scales (and zero points) of the four output columns 4 * (lane / 16) .. + 3 of tile `tile` in group `grp`.
-template <int KIND>
-__device__ __forceinline__ void w4_params4(const W4Args& a, int64_t tile, int grp, int quad, f32x4& s, f32x4& sz) {
-  const int64_t at = (tile * a.gp + grp) * 16 + quad * 4;
-  if constexpr (KIND == W4_U4) {
-    const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const uint32_t*>(a.params) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = (float)h_from_bits(v[i]);
-      sz[i] = s[i] * (float)h_from_bits(v[i] >> 16);  // exact: 11 x 11 bits
-    }
-  } else {
-    const u32x2 v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.params) + at);
-    s[0] = (float)h_from_bits(v[0]);
-    s[1] = (float)h_from_bits(v[0] >> 16);
-    s[2] = (float)h_from_bits(v[1]);
-    s[3] = (float)h_from_bits(v[1] >> 16);
-  }
-}
-
 template <class T> __device__ __forceinline__ void w4_store4(uint16_t* y, int64_t nc, int64_t row, int64_t col, f32x4 v) {
   uint16_t* to = y + row * nc + col;
   if (nc % 4 == 0) {  // (y itself is 16-byte aligned)
@@ -67,28 +47,25 @@ template <class T> __device__ __forceinline__ void w4_store4(uint16_t* y, int64_
       if (col + i < nc) to[i] = T::from_f32(v[i]);
   }
 }
-template <class T>
-__device__ __forceinline__ f32x4 w4_bias4(const uint16_t* bias, int64_t nc, int expert, int64_t col, f32x4 v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i < nc) v[i] += T::to_f32(bias[expert * nc + col + i]);
-  return v;
-}
-
 // ---- few rows --------------------------------------------------------------------------------------
 // A workgroup owns NT column tiles and 16 * MT rows; its waves take the 128-blocks of the contraction in turn and their
-// sums meet in LDS at the end, in the waves' order.  The weight is the matrix instruction's A operand, so a lane's four
-// results are four neighbouring columns of one row and y is stored 8 bytes at a time.
+// sums meet in LDS at the end, in the waves' order.  Everything is in registers on its way: a wave keeps D blocks in
+// flight while it works on the D before them.  Rows that are not there repeat the tile's last one (their loads fall into
+// the same lines, their results are not stored; masking them off measured slower).  Rows are 16-byte aligned and a multiple of 128 long (k_w4_pad).
+template <class T, int KIND, int MT, int NT, int FS, int D> struct W4RowsStage {
+  u32x4 w[D][NT], x[D][MT][4];
+  uint32_t s[D][NT];  // lane 16 v + c: the scale (and zero point) of column c in window v of the block's 4 / FS
+};
 template <class T, int KIND, int MT, int NT, int FS>
-__global__ __launch_bounds__(512) void k_w4_rows(const W4Args a, const W4Product p) {
+__global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_w4_rows(const W4Args a, const W4Product p) {
   extern __shared__ f32x4 w4_red[];
-  constexpr int D = MT * NT >= 4 ? 1 : 2;  // 128-blocks in flight per wave
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int quad = lane >> 4;
-  const int64_t tile0 = (int64_t)(blockIdx.x % p.nblocks) * NT;
+  constexpr int D = MT * NT >= 4 ? 1 : 2, W = 4 / FS;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+  const int quad = lane >> 4, l16 = lane & 15;
+  const int tile0 = (int)(blockIdx.x % (uint32_t)p.nblocks) * NT;
   int expert, rows;
   int64_t row0;
-  if (!w4_find_tile(a, 16 * MT, blockIdx.x / p.nblocks, expert, row0, rows)) return;
+  if (!w4_find_tile(a, 16 * MT, (int)(blockIdx.x / (uint32_t)p.nblocks), expert, row0, rows)) return;
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -96,38 +73,53 @@ __global__ __launch_bounds__(512) void k_w4_rows(const W4Args a, const W4Product
     for (int n = 0; n < NT; ++n) acc[m][n] = {0, 0, 0, 0};
 
   if (expert >= 0) {
-    int64_t tile[NT];
+    const uint32_t* wp[NT];
+    int64_t sp[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) tile[n] = (int64_t)expert * a.nt + (tile0 + n < a.nt ? tile0 + n : a.nt - 1);
-    const uint16_t* xr[MT];
-    bool live[MT];
+    for (int n = 0; n < NT; ++n) {
+      const int64_t tile = (int64_t)expert * a.nt + (tile0 + n < a.nt ? tile0 + n : a.nt - 1);
+      wp[n] = p.b + tile * a.kt * 256;
+      sp[n] = tile * a.gp * 16;
+    }
+    const uint16_t* xp = p.x + row0 * p.ldx;
+    uint32_t xo[MT];  // (rows of a tile lie within 2^31 bytes: others are copied first)
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int r = m * 16 + (lane & 15);
-      live[m] = r < rows;
-      xr[m] = p.x + (row0 + (live[m] ? r : 0)) * p.ldx;
+      const int r = m * 16 + l16;
+      xo[m] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.ldx + quad * 8;
     }
-    for (int kb = w; kb < a.kt; kb += nw * D) {
-      u32x4 wv[D][NT], xv[D][MT][4];
+    typedef W4RowsStage<T, KIND, MT, NT, FS, D> Stage;
+    auto load = [&](Stage& g, int kb, int n_blocks) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        const int k0 = kb + d * nw;
-        if (k0 < a.kt) {
+        if (d < n_blocks) {
+          const int k0 = kb + d * nw;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) wv[d][n] = *reinterpret_cast<const u32x4*>(p.b + (tile[n] * a.kt + k0) * 256 + lane * 4);
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              xv[d][m][j] = {0, 0, 0, 0};
-              if (live[m]) xv[d][m][j] = w4_load8(xr[m], (int64_t)k0 * 128 + j * 32 + quad * 8, p.kc, p.vec);
-            }
+          for (int n = 0; n < NT; ++n) {
+            g.w[d][n] = *reinterpret_cast<const u32x4*>(wp[n] + (int64_t)k0 * 256 + lane * 4);
+            // one load for all windows of the block: it would take as long as a load of the weight for each
+            const int64_t at = sp[n] + l16 + (W == 1 ? w4_group(a, k0 * 4) : w4_group(a, k0 * 4 + (quad & (W - 1)) * FS)) * 16;
+            if constexpr (KIND == W4_U4)
+              g.s[d][n] = static_cast<const uint32_t*>(a.params)[at];
+            else
+              g.s[d][n] = static_cast<const uint16_t*>(a.params)[at];
+          }
         }
       }
 #pragma unroll
+      for (int d = 0; d < D; ++d)
+        if (d < n_blocks) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              g.x[d][m][j] = *reinterpret_cast<const u32x4*>(xp + (int64_t)(kb + d * nw) * 128 + j * 32 + xo[m]);
+        }
+    };
+    auto work = [&](const Stage& g, int n_blocks) {
+#pragma unroll
       for (int d = 0; d < D; ++d) {
-        const int k0 = kb + d * nw;
-        if (k0 < a.kt) {
+        if (d < n_blocks) {
           f32x4 tmp[MT][NT], xs[MT];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -141,49 +133,77 @@ __global__ __launch_bounds__(512) void k_w4_rows(const W4Args a, const W4Product
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const u32x4 v = w4_decode<T, KIND>(wv[d][n][j], a.lut);
+              const u32x4 v = w4_decode<T, KIND>(g.w[d][n][j], a.lut);
 #pragma unroll
-              for (int m = 0; m < MT; ++m) tmp[m][n] = T::mfma(v, xv[d][m][j], tmp[m][n]);
+              for (int m = 0; m < MT; ++m) tmp[m][n] = T::mfma(g.x[d][m][j], v, tmp[m][n]);
             }
-            if constexpr (KIND == W4_U4) {
+            if constexpr (KIND == W4_U4) {  // sums of x, in the layout of the results
               const u32x4 ones = {T::kOnes, T::kOnes, T::kOnes, T::kOnes};
 #pragma unroll
-              for (int m = 0; m < MT; ++m) xs[m] = T::mfma(ones, xv[d][m][j], xs[m]);
+              for (int m = 0; m < MT; ++m) xs[m] = T::mfma(g.x[d][m][j], ones, xs[m]);
             }
             if ((j + 1) % FS == 0) {
-              const int grp = w4_group(a, k0 * 4 + j);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                f32x4 s, sz;
-                w4_params4<KIND>(a, tile[n], grp, quad, s, sz);
+                const uint32_t sv = W == 1 ? g.s[d][n] : (uint32_t)__builtin_amdgcn_ds_bpermute((j / FS * 16 + l16) * 4, (int)g.s[d][n]);
+                const float s = (float)h_from_bits(sv);
+                const float sz = KIND == W4_U4 ? -(s * (float)h_from_bits(sv >> 16)) : 0.0f;  // exact: 11 x 11 bits
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
-                    acc[m][n][i] = __builtin_fmaf(s[i], tmp[m][n][i], acc[m][n][i]);
-                    if constexpr (KIND == W4_U4) acc[m][n][i] = __builtin_fmaf(-sz[i], xs[m][i], acc[m][n][i]);
+                    acc[m][n][i] = __builtin_fmaf(s, tmp[m][n][i], acc[m][n][i]);
+                    if constexpr (KIND == W4_U4) acc[m][n][i] = __builtin_fmaf(sz, xs[m][i], acc[m][n][i]);
                   }
               }
             }
           }
         }
       }
+    };
+    const int first = (int)((int64_t)a.kt * blockIdx.y / p.splits), last = (int)((int64_t)a.kt * (blockIdx.y + 1) / p.splits);
+    int left = (last - first - w + nw - 1) / nw;  // this wave's blocks
+    int kb = first + w;
+    Stage g0, g1;
+    if (left >= D) load(g0, kb, D);
+    while (left >= D) {
+      left -= D;
+      kb += D * nw;
+      const bool more = left >= D;
+      if (more) load(g1, kb, D);
+      work(g0, D);
+      if (!more) break;
+      left -= D;
+      kb += D * nw;
+      if (left >= D) load(g0, kb, D);
+      work(g1, D);
+    }
+    if (D > 1 && left > 0) {  // D is at most 2: one block
+      load(g0, kb, 1);
+      work(g0, 1);
     }
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) w4_red[((w * MT + m) * NT + n) * 64 + lane] = acc[m][n];
+    for (int n = 0; n < NT; ++n)
+      if (m * 16 + quad * 4 < rows) w4_red[((w * MT + m) * NT + n) * 64 + lane] = acc[m][n];
   __syncthreads();
-  for (int i = threadIdx.x; i < MT * NT * 64; i += blockDim.x) {
-    f32x4 v = w4_red[i];
-    for (int o = 1; o < nw; ++o) v += w4_red[o * MT * NT * 64 + i];
-    const int l = i & 63, n = (i >> 6) % NT, m = (i >> 6) / NT;
-    const int r = m * 16 + (l & 15);
-    const int64_t col = (tile0 + n) * 16 + (l >> 4) * 4;
-    if (r < rows && col < p.nc) {
-      if (p.bias && expert >= 0) v = w4_bias4<T>(p.bias, p.nc, expert, col, v);
-      w4_store4<T>(p.y, p.nc, row0 + r, col, v);
+  // one thread per result; column 16 n + c of row r: lane 16 (r % 16 / 4) + c, component r % 4
+  const float* red = reinterpret_cast<const float*>(w4_red);
+  for (int i = threadIdx.x; i < rows * NT * 16; i += blockDim.x) {
+    const int c = i % (NT * 16), r = i / (NT * 16);
+    const int64_t col = (int64_t)tile0 * 16 + c;
+    const float* from = red + ((((r >> 4) * NT + (c >> 4)) * 64 + ((r & 15) >> 2) * 16 + (c & 15)) << 2) + (r & 3);
+    float v = from[0];
+#pragma unroll 4
+    for (int o = 1; o < nw; ++o) v += from[o * MT * NT * 256];
+    if (col < p.nc) {
+      if (p.bias && expert >= 0 && blockIdx.y == 0) v += T::to_f32(p.bias[expert * p.nc + col]);
+      if (p.part)
+        p.part[((int64_t)blockIdx.y * a.rows + row0 + r) * (p.ct * 16) + col] = v;
+      else
+        p.y[(row0 + r) * p.nc + col] = T::from_f32(v);
     }
   }
 }
@@ -241,21 +261,28 @@ template <int KIND> struct W4Scales<W4BF16, KIND> {
 // GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.
 // GRAD = true (dx = dy W, operand b transposed): scales change along the contraction, so they are multiplied into the
 // weights, which are rounded once to T -- half a step of T per weight, as a weight stored in T has.
+template <int NT, int W> struct W4Ahead {  // what a wave holds of a block that is on its way
+  u32x4 b[NT][2];
+  uint32_t s[NT][W];
+};
 typedef __attribute__((address_space(1))) const void w4_global_t;
 typedef __attribute__((address_space(3))) void w4_lds_t;
 
 template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int FS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, const W4Product p) {
   constexpr int BM = 32 * MT * WM, NW = WM * WN, CH = BM / 4 / NW;  // 1 KiB pieces (4 rows) per wave
-  static_assert(BM / 4 % NW == 0, "the rows of a block are dealt evenly");
+  constexpr int W = 4 / FS;                                         // windows of a block with a scale each
+  constexpr bool XS = KIND == W4_U4 && !GRAD;
+  static_assert(BM / 4 % NW == 0 && BM % 64 == 0, "the rows of a block are dealt evenly");
   __shared__ u32x4 lds[2][BM * 16];
+  __shared__ f32x4 lds_xs[XS ? 2 : 1][XS ? W * BM / 4 : 1];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
   const int wm = w % WM, wn = w / WM;
   const int64_t mb = blockIdx.x % p.mblocks;
   const int64_t tile0 = ((int64_t)(blockIdx.x / p.mblocks) * WN + wn) * NT;  // tiles of 32 columns
   int expert, rows;
   int64_t row0;
-  if (!w4_find_tile(a, BM, mb, expert, row0, rows)) return;
+  if (!w4_find_tile(a, BM, (int)mb, expert, row0, rows)) return;
   f32x16 acc[MT][NT];     // GRAD: the matrix instructions' own sums
   float sum[MT][NT][16];  // forward: the scaled sums (single registers: they are never a matrix operand)
 #pragma unroll
@@ -291,64 +318,81 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
       const int64_t c = tile0 + n, last = (p.ct - 1) >> 1;
       st0[n] = ((int64_t)expert * a.gp + w4_group(a, (int)(c < last ? c : last))) * p.rb * 128 + half * 8;
     }
-    u32x4 bn[NT][2];
-    auto fetch = [&](int kb, int buf) {
+    W4Ahead<NT, GRAD ? 1 : W> next;
+    auto fetch = [&](int kb, int buf, W4Ahead<NT, GRAD ? 1 : W>& to) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
         __builtin_amdgcn_global_load_lds((w4_global_t*)(xp[c] + (int64_t)kb * 128), (w4_lds_t*)&lds[buf][(w * CH + c) * 64], 16, 0, 0);
+      if constexpr (XS) {  // 64 row sums to a wave's load; a tile may read past the last row
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int c = 0; c < W * BM / 64; ++c)
+          if (c % NW == w)
+            __builtin_amdgcn_global_load_lds((w4_global_t*)(p.xs + ((int64_t)kb * W + c / (BM / 64)) * a.rows + row0 + c % (BM / 64) * 64 + lane),
+                                             (w4_lds_t*)&lds_xs[buf][c * 16], 4, 0, 0);
+      }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) bn[n][h] = *reinterpret_cast<const u32x4*>(bp[n] + (int64_t)kb * 256 + h * 128);
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) to.b[n][h] = *reinterpret_cast<const u32x4*>(bp[n] + (int64_t)kb * 256 + h * 128);
+        if constexpr (!GRAD) {
+#pragma unroll
+          for (int v = 0; v < W; ++v) {
+            const int64_t at = pt[n] + w4_group(a, kb * 4 + v * FS) * 16;
+            if constexpr (KIND == W4_U4)
+              to.s[n][v] = static_cast<const uint32_t*>(a.params)[at];
+            else
+              to.s[n][v] = static_cast<const uint16_t*>(a.params)[at];
+          }
+        }
+      }
     };
-    if (kb0 < kb1) fetch(kb0, 0);
+    if (kb0 < kb1) fetch(kb0, 0, next);
     __syncthreads();
     for (int kb = kb0; kb < kb1; ++kb) {
       const int buf = (kb - kb0) & 1;
-      u32x4 bv[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) bv[n][0] = bn[n][0], bv[n][1] = bn[n][1];
-      if (kb + 1 < kb1) fetch(kb + 1, buf ^ 1);
+      const W4Ahead<NT, GRAD ? 1 : W> cur = next;
+      if (kb + 1 < kb1) fetch(kb + 1, buf ^ 1, next);
       const u32x4* xb = lds[buf] + (wm * MT * 32 + l32) * 16;
       const int turn = (l32 & 15) ^ half;
+      // One row tile: its operands of the whole block at once, since two products hide no LDS load.
+      u32x4 xa[MT == 1 ? 8 : 1];
+      if constexpr (MT == 1) {
+#pragma unroll
+        for (int st = 0; st < 8; ++st) xa[st] = xb[(2 * st) ^ turn];
+      }
       if constexpr (!GRAD) {
         f32x16 tmp[MT][NT];
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
           u32x4 xv[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) xv[m] = xb[m * 512 + ((2 * st) ^ turn)];
+          for (int m = 0; m < MT; ++m) xv[m] = MT == 1 ? xa[MT == 1 ? st : 0] : xb[m * 512 + ((2 * st) ^ turn)];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const u32x4 v = w4_decode<T, KIND>(bv[n][st & 1][st >> 1], a.lut);
+            const u32x4 v = w4_decode<T, KIND>(cur.b[n][st & 1][st >> 1], a.lut);
 #pragma unroll
             for (int m = 0; m < MT; ++m) tmp[m][n] = T::mfma32(xv[m], v, st % (2 * FS) == 0 ? w4_zero16() : tmp[m][n]);
           }
           if ((st + 1) % (2 * FS) == 0) {
-            const int grp = w4_group(a, kb * 4 + st / 2);
+            const int v = st / (2 * FS);
             float s[NT], sz[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              if constexpr (KIND == W4_U4) {
-                const uint32_t v = static_cast<const uint32_t*>(a.params)[pt[n] + grp * 16];
-                s[n] = (float)h_from_bits(v);
-                sz[n] = -(s[n] * (float)h_from_bits(v >> 16));  // exact: 11 x 11 bits
-              } else {
-                s[n] = (float)h_from_bits(static_cast<const uint16_t*>(a.params)[pt[n] + grp * 16]);
-              }
+              s[n] = (float)h_from_bits(cur.s[n][v]);
+              if constexpr (KIND == W4_U4) sz[n] = -(s[n] * (float)h_from_bits(cur.s[n][v] >> 16));  // exact: 11 x 11 bits
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              const float* xs = KIND == W4_U4 ? p.xs + (int64_t)(kb * (4 / FS) + st / (2 * FS)) * a.rows + row0 + (wm * MT + m) * 32 + half * 4 : nullptr;
 #pragma unroll
               for (int q = 0; q < 4; ++q) {  // registers 4 q .. 4 q + 3: rows 8 q + 4 half + (0 .. 3) of the tile
+                f32x4 x = {0, 0, 0, 0};
+                if constexpr (XS) x = lds_xs[buf][v * (BM / 4) + (wm * MT + m) * 8 + q * 2 + half];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const float x = KIND == W4_U4 ? xs[q * 8 + i] : 0.0f;
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     sum[m][n][4 * q + i] = __builtin_fmaf(s[n], tmp[m][n][4 * q + i], sum[m][n][4 * q + i]);
-                    if constexpr (KIND == W4_U4) sum[m][n][4 * q + i] = __builtin_fmaf(sz[n], x, sum[m][n][4 * q + i]);
+                    if constexpr (KIND == W4_U4) sum[m][n][4 * q + i] = __builtin_fmaf(sz[n], x[i], sum[m][n][4 * q + i]);
                   }
                 }
               }
@@ -366,10 +410,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
           for (int g = 0; g < SETS; ++g) sc[g].load(p, st0[g] + kb * 128 + st * 16);
           u32x4 xv[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) xv[m] = xb[m * 512 + ((2 * st) ^ turn)];
+          for (int m = 0; m < MT; ++m) xv[m] = MT == 1 ? xa[MT == 1 ? st : 0] : xb[m * 512 + ((2 * st) ^ turn)];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const u32x4 v = sc[FS == 1 ? n : 0].scaled(bv[n][st & 1][st >> 1], a.lut);
+            const u32x4 v = sc[FS == 1 ? n : 0].scaled(cur.b[n][st & 1][st >> 1], a.lut);
 #pragma unroll
             for (int m = 0; m < MT; ++m) acc[m][n] = T::mfma32(xv[m], v, acc[m][n]);
           }
@@ -462,7 +506,7 @@ struct W4Plan {
 
 template <class T, int KIND, int MT, int NT>
 static void w4_rows_go(const W4Args& a, const W4Product& p, const W4Plan& pl, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)p.nblocks * p.mblocks)), block(64 * pl.waves);
+  const dim3 grid((unsigned)((int64_t)p.nblocks * p.mblocks), p.splits), block(64 * pl.waves);
   const size_t lds = (size_t)pl.waves * MT * NT * 1024;
   if (pl.fs == 4)
     hipLaunchKernelGGL((k_w4_rows<T, KIND, MT, NT, 4>), grid, block, lds, st, a, p);
@@ -492,13 +536,14 @@ template <class T, int KIND>
 hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool grad, hipStream_t st) {
   if (!pl.bm) {
     if (pl.mt == 1 && pl.nt == 1) w4_rows_go<T, KIND, 1, 1>(a, p, pl, st);
+    else if (pl.mt == 1 && pl.nt == 2) w4_rows_go<T, KIND, 1, 2>(a, p, pl, st);
     else if (pl.mt == 1) w4_rows_go<T, KIND, 1, 4>(a, p, pl, st);
     else if (pl.nt == 1) w4_rows_go<T, KIND, 2, 1>(a, p, pl, st);
+    else if (pl.nt == 2) w4_rows_go<T, KIND, 2, 2>(a, p, pl, st);
     else w4_rows_go<T, KIND, 2, 4>(a, p, pl, st);
   } else if (grad) {
     if (pl.bm == 64) w4_gemm_go<T, KIND, true, 1, 2, 2, 2>(a, p, pl, st);
-    else if (pl.bn == 256) w4_gemm_go<T, KIND, true, 4, 2, 1, 4>(a, p, pl, st);
-    else w4_gemm_go<T, KIND, true, 2, 2, 2, 2>(a, p, pl, st);
+    else w4_gemm_go<T, KIND, true, 4, 2, 1, 4>(a, p, pl, st);
   } else {
     if (pl.bm == 64) w4_gemm_go<T, KIND, false, 1, 2, 2, 2>(a, p, pl, st);
     else w4_gemm_go<T, KIND, false, 2, 2, 2, 2>(a, p, pl, st);

@@ -113,9 +113,11 @@ class PackedWeight:
             s.values[:] = values
         self._c = s
         self._ref = ctypes.byref(s)
+        self._need = {}   # workspace bytes by (rows, aligned, counted, grad)
+        self._device = self.data.device
 
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref")}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref", "_need", "_device")}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
@@ -123,7 +125,7 @@ class PackedWeight:
 
     @property
     def device(self):
-        return self.data.device
+        return self._device
 
     @property
     def shape(self):
@@ -257,26 +259,40 @@ def _rows_of(t):
 
 def _product(t, weight, bias, counts, grad):
     """One launch of mq_linear4 (grad: mq_linear4_grad) on rows t [R, K] ([R, N])."""
-    L = _bind()
+    L = _bound or _bind()
     rows = t.shape[0]
-    out = torch.empty(rows, weight.k if grad else weight.n, dtype=t.dtype, device=t.device)
+    out = t.new_empty((rows, weight.k if grad else weight.n))
     if not rows:
         return out
     t, ld = _rows_of(t)
+    index = t.device.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _launch(L, t, ld, rows, weight, bias, counts, grad, out, index)
+    return _launch(L, t, ld, rows, weight, bias, counts, grad, out, index)
+
+
+def _launch(L, t, ld, rows, weight, bias, counts, grad, out, index):
+    x = t.data_ptr()
+    aligned = x % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 25 or rows == 1)
+    key = (rows, aligned, counts is not None, grad)
+    need = weight._need.get(key)
+    if need is None:
+        if len(weight._need) >= 4096:
+            weight._need.clear()
+        need = weight._need[key] = L.mq_linear4_workspace_bytes(weight._ref, *key)
+    # of this call alone: a captured graph keeps it in its own pool, and calls on other streams have their own
+    ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
+    wp = None if ws is None else ws.data_ptr()
     cp = None if counts is None else counts.data_ptr()
-    with torch.cuda.device(t.device):
-        aligned = t.data_ptr() % 16 == 0 and (ld % 8 == 0 or rows == 1)
-        need = L.mq_linear4_workspace_bytes(weight._ref, rows, aligned, counts is not None, grad)
-        # of this call alone: a captured graph keeps it in its own pool, and calls on other streams have their own
-        ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
-        wp = None if ws is None else ws.data_ptr()
-        stream = torch.cuda.current_stream().cuda_stream
-        if grad:
-            rc = L.mq_linear4_grad(weight._ref, t.data_ptr(), _XDTYPES[t.dtype], rows, ld, cp, out.data_ptr(), wp, need, stream)
-        else:
-            rc = L.mq_linear4(weight._ref, t.data_ptr(), _XDTYPES[t.dtype], rows, ld, None if bias is None else bias.data_ptr(),
-                              cp, out.data_ptr(), wp, need, stream)
-    _lib.check(rc)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if grad:
+        rc = L.mq_linear4_grad(weight._ref, x, _XDTYPES[t.dtype], rows, ld, cp, out.data_ptr(), wp, need, stream)
+    else:
+        rc = L.mq_linear4(weight._ref, x, _XDTYPES[t.dtype], rows, ld, None if bias is None else bias.data_ptr(), cp,
+                          out.data_ptr(), wp, need, stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -317,9 +333,9 @@ def _check_operands(x, weight, bias):
         raise RuntimeError("packed products expect ROCm device tensors; no CPU fallback exists")
     if x.dtype not in _XDTYPES:
         raise ValueError(f"float16 or bfloat16 activations are wanted, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != weight.k:
+    if not x.dim() or x.shape[-1] != weight.k:
         raise ValueError(f"activations {tuple(x.shape)} do not fit a weight {tuple(weight.shape)}")
-    if x.device != weight.device:
+    if x.device != weight._device:
         raise ValueError(f"activations on {x.device}, weight on {weight.device}")
     if bias is not None:
         want = (weight.n,) if weight.experts is None else (weight.experts, weight.n)
