@@ -617,8 +617,8 @@ int mq_histogram(const void* x, int32_t dtype, int64_t n, const double* edges, i
  *
  *   W[e][n][k] = scale[e][n][k / group] * (q[e][n][k] - zero[e][n][k / group])
  *   mq_linear4       y[r]  = x[r]  W[e(r)]^T + bias[e(r)]
- *   mq_linear4_grad  dx[r] = dy[r] W[e(r)]            (the weight is frozen: no gradient of codes or scales)
- *   mq_bias_grad     db[e] = sum of dy[r] over the rows of e
+ *   mq_linear4_grad  dx[r] = dy[r] W[e(r)],  db[e] = sum of dy[r] over the rows of e
+ *                                                    (the weight is frozen: no gradient of codes or scales)
  *
  * x, dy, bias: float16 or bfloat16, y / dx of the same type, sums in float32, one rounding at the end.  In mq_linear4
  * the codes' values enter the matrix cores exactly and the scales are applied in float32.  In mq_linear4_grad the scales
@@ -662,16 +662,14 @@ int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream);
 
 /* May be 0.  aligned: every row of x (dy) starts on a multiple of 16 bytes and the next one at most 2^25 elements on;
  * other rows are copied first.
- * counted: counts will be given; grad: for mq_linear4_grad. */
+ * counted: counts will be given; grad: 0 for mq_linear4, for mq_linear4_grad 1 (dx), 2 (db) or 3 (both). */
 size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t aligned, int32_t counted, int32_t grad);
 /* x [rows][ldx] (ldx elements from row to row, 0 = the same row again), y [rows][n] contiguous, 16-byte aligned. */
 int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
                const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream);
+/* dx and / or db (either may be NULL, not both): db [experts][n] in the type of dy, summed in float32. */
 int mq_linear4_grad(const mq_w4* w, const void* dy, int32_t dtype, int64_t rows, int64_t ldy, const int32_t* counts,
-                    void* dx, void* workspace, size_t workspace_bytes, void* hip_stream);
-size_t mq_bias_grad_workspace_bytes(int64_t rows, int64_t n, int64_t experts);
-int mq_bias_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ldy, int64_t experts,
-                 const int32_t* counts, void* db, void* workspace, size_t workspace_bytes, void* hip_stream);
+                    void* dx, void* db, void* workspace, size_t workspace_bytes, void* hip_stream);
 
 #ifdef __cplusplus
 }

@@ -227,18 +227,18 @@ template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args
 }
 
 // ---- the bias's gradient -----------------------------------------------------------------------------
-// Sums of dy's rows per expert in float32: 64 columns per workgroup, an expert's rows cut into `splits` runs whose sums
-// a second launch adds in order.
+// Sums of dy's rows per expert in float32: 64 columns to a workgroup, whose sixteen waves take the rows in turn; where an
+// expert has many rows they are cut into runs, whose sums a second launch adds in order.  Bound by reading dy once more.
 struct BiasArgs {
   const uint16_t* dy;
   const int32_t* counts;
-  float* part;  // [splits][E][N]
+  float* part;  // [splits][E][N], NULL when splits == 1
   uint16_t* db;
   int64_t rows, n, ldy, experts;
   int32_t splits;
 };
-template <class T> __global__ __launch_bounds__(256) void k_w4_bias(const BiasArgs p) {
-  __shared__ float red[4][64];
+template <class T> __global__ __launch_bounds__(1024) void k_w4_bias(const BiasArgs p) {
+  __shared__ float red[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t col = (int64_t)blockIdx.x * 64 + lane, e = blockIdx.z;
   int64_t start = 0, count = p.rows;
@@ -253,19 +253,27 @@ template <class T> __global__ __launch_bounds__(256) void k_w4_bias(const BiasAr
   const int64_t r0 = start + count * blockIdx.y / p.splits, r1 = start + count * (blockIdx.y + 1) / p.splits;
   float s = 0;
   if (col < p.n) {
-#pragma unroll 4
-    for (int64_t r = r0 + w; r < r1; r += 4) s += T::to_f32(p.dy[r * p.ldy + col]);
+    const uint16_t* from = p.dy + col;
+#pragma unroll 8
+    for (int64_t r = r0 + w; r < r1; r += 16) s += T::to_f32(from[r * p.ldy]);
   }
   red[w][lane] = s;
   __syncthreads();
-  if (w == 0 && col < p.n)
-    p.part[((int64_t)blockIdx.y * p.experts + e) * p.n + col] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+  if (w == 0 && col < p.n) {
+    float v = red[0][lane];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += red[i][lane];
+    if (p.part)
+      p.part[((int64_t)blockIdx.y * p.experts + e) * p.n + col] = v;
+    else
+      p.db[e * p.n + col] = T::from_f32(v);
+  }
 }
 template <class T> __global__ __launch_bounds__(256) void k_w4_bias_join(const BiasArgs p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = p.experts * p.n;
   if (i >= total) return;
-  float s = 0;
-  for (int o = 0; o < p.splits; ++o) s += p.part[o * total + i];
+  float s = p.part[i];
+  for (int o = 1; o < p.splits; ++o) s += p.part[o * total + i];
   p.db[i] = T::from_f32(s);
 }
 
@@ -397,6 +405,21 @@ size_t sums_bytes(const mq_w4* w, const W4Plan& pl, const W4Product& p, int64_t 
   return pl.bm && !grad && w->kind == W4_U4 ? up256(((size_t)p.rb * (4 / pl.fs) * rows + pl.bm) * 4) : 0;  // (a tile reads past the last row)
 }
 
+int32_t bias_splits(int64_t rows, int64_t experts) {
+  const int64_t per = rows / experts;  // up to 512 rows in one run: a second launch costs as much as reading them
+  return (int32_t)(per <= 512 ? 1 : per / 256 < 32 ? per / 256 : 32);
+}
+size_t bias_bytes(const mq_w4* w, int64_t rows) {
+  const int32_t s = bias_splits(rows, w->experts);
+  return s > 1 ? up256((size_t)s * w->experts * w->n * 4) : 0;
+}
+template <class T> hipError_t bias_launch(const BiasArgs& p, hipStream_t st) {
+  hipLaunchKernelGGL((k_w4_bias<T>), dim3((unsigned)((p.n + 63) / 64), p.splits, (unsigned)p.experts), dim3(1024), 0, st, p);
+  if (p.part)
+    hipLaunchKernelGGL((k_w4_bias_join<T>), dim3((unsigned)((p.experts * p.n + 255) / 256)), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
 int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
             const int32_t* counts, void* y, void* ws, size_t ws_bytes, void* stream, bool grad) {
   int rc = check_w4(w);
@@ -420,7 +443,7 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   const size_t padded = !p.vec || kc % 128 || (ldx > kMaxStride && rows > 1) ? (size_t)rows * p.rb * 256 : 0;
   const size_t need = turned + part_bytes(p, rows) + padded;
   if (need && (!ws || ws_bytes < need)) return MQ_ERR_WORKSPACE;
-  if (need && (uintptr_t)ws % 16) return MQ_ERR_ALIGN;
+  if ((uintptr_t)ws % 16) return MQ_ERR_ALIGN;
   p.x = static_cast<const uint16_t*>(x);
   p.ldx = ldx;
   p.b = a.data;
@@ -467,11 +490,6 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
     return MQ_ERR_HIP;
   }
   return MQ_OK;
-}
-
-int32_t bias_splits(int64_t rows, int64_t experts) {
-  const int64_t s = rows / (experts < 1 ? 1 : experts) / 64;
-  return (int32_t)(s < 1 ? 1 : s > 32 ? 32 : s);
 }
 
 }  // namespace
@@ -559,42 +577,43 @@ extern "C" int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream) {
 }
 extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t aligned, int32_t counted, int32_t grad) {
   if (check_w4(w) != MQ_OK || rows < 1 || rows > kMaxRows) return 0;
+  size_t need = grad & 2 ? bias_bytes(w, rows) : 0;
+  if (grad == 2) return need;
   W4Product p = {};
   const W4Plan pl = plan_of(w, rows, grad != 0, counted != 0, &p);
-  return (grad ? turn_bytes(w) : sums_bytes(w, pl, p, rows, false)) + part_bytes(p, rows) +
-         (!aligned || p.kc % 128 ? (size_t)rows * p.rb * 256 : 0);
+  need += (grad ? turn_bytes(w) : sums_bytes(w, pl, p, rows, false)) + part_bytes(p, rows);
+  return need + (!aligned || p.kc % 128 ? (size_t)rows * p.rb * 256 : 0);
 }
 extern "C" int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
                           const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream) {
   return product(w, x, dtype, rows, ldx, bias, counts, y, workspace, workspace_bytes, hip_stream, false);
 }
 extern "C" int mq_linear4_grad(const mq_w4* w, const void* dy, int32_t dtype, int64_t rows, int64_t ldy,
-                               const int32_t* counts, void* dx, void* workspace, size_t workspace_bytes, void* hip_stream) {
-  return product(w, dy, dtype, rows, ldy, nullptr, counts, dx, workspace, workspace_bytes, hip_stream, true);
-}
-extern "C" size_t mq_bias_grad_workspace_bytes(int64_t rows, int64_t n, int64_t experts) {
-  if (rows < 0 || n < 1 || experts < 1) return 0;
-  return (size_t)bias_splits(rows, experts) * experts * n * 4;
-}
-extern "C" int mq_bias_grad(const void* dy, int32_t dtype, int64_t rows, int64_t n, int64_t ldy, int64_t experts,
-                            const int32_t* counts, void* db, void* workspace, size_t workspace_bytes, void* hip_stream) {
-  if (rows < 0 || n < 1 || experts < 1 || ldy < 0 || (!counts && experts != 1) || !db || (rows > 0 && !dy)) return MQ_ERR_ARG;
-  if (dtype != MQ_F16 && dtype != MQ_BF16) return MQ_ERR_UNSUPPORTED;
-  if (rows > kMaxRows || n > kMaxN || experts > kMaxExperts) return MQ_ERR_TOO_LARGE;
-  if ((uintptr_t)dy % 2 || (uintptr_t)db % 2 || (uintptr_t)counts % 4 || (uintptr_t)workspace % 4) return MQ_ERR_ALIGN;
-  if (!workspace || workspace_bytes < mq_bias_grad_workspace_bytes(rows, n, experts)) return MQ_ERR_WORKSPACE;
-  BiasArgs p = {static_cast<const uint16_t*>(dy), counts, static_cast<float*>(workspace), static_cast<uint16_t*>(db),
-                rows, n, ldy, experts, bias_splits(rows, experts)};
-  hipStream_t st = static_cast<hipStream_t>(hip_stream);
-  const dim3 grid((unsigned)((n + 63) / 64), p.splits, (unsigned)experts), join((unsigned)((experts * n + 255) / 256));
-  if (dtype == MQ_F16) {
-    hipLaunchKernelGGL((k_w4_bias<W4F16>), grid, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((k_w4_bias_join<W4F16>), join, dim3(256), 0, st, p);
-  } else {
-    hipLaunchKernelGGL((k_w4_bias<W4BF16>), grid, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((k_w4_bias_join<W4BF16>), join, dim3(256), 0, st, p);
+                               const int32_t* counts, void* dx, void* db, void* workspace, size_t workspace_bytes,
+                               void* hip_stream) {
+  int rc = check_w4(w);
+  if (rc != MQ_OK) return rc;
+  if (!dx && !db) return MQ_ERR_ARG;
+  size_t used = 0;
+  if (db) {
+    if (dtype != MQ_F16 && dtype != MQ_BF16) return MQ_ERR_UNSUPPORTED;
+    if (rows < 0 || ldy < 0 || (rows > 0 && !dy) || (!counts && w->experts != 1)) return MQ_ERR_ARG;
+    if (rows > kMaxRows) return MQ_ERR_TOO_LARGE;
+    if ((uintptr_t)dy % 2 || (uintptr_t)db % 2 || (uintptr_t)counts % 4 || (uintptr_t)workspace % 16) return MQ_ERR_ALIGN;
+    used = bias_bytes(w, rows);
+    if (used && (!workspace || workspace_bytes < used)) return MQ_ERR_WORKSPACE;
   }
-  MQ_HIP(hipGetLastError());
+  if (dx) {
+    rc = product(w, dy, dtype, rows, ldy, nullptr, counts, dx, static_cast<char*>(workspace) + used, workspace_bytes - used,
+                 hip_stream, true);
+    if (rc != MQ_OK) return rc;
+  }
+  if (db) {
+    const BiasArgs p = {static_cast<const uint16_t*>(dy), counts, used ? static_cast<float*>(workspace) : nullptr,
+                        static_cast<uint16_t*>(db), rows, w->n, ldy, w->experts, bias_splits(rows, w->experts)};
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    MQ_HIP(dtype == MQ_F16 ? bias_launch<W4F16>(p, st) : bias_launch<W4BF16>(p, st));
+  }
   return MQ_OK;
 }
 #endif

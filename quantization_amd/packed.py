@@ -46,9 +46,7 @@ def _bind():
         L.mq_w4_unpack.restype, L.mq_w4_unpack.argtypes = ctypes.c_int, [pw, vp, vp]
         L.mq_linear4_workspace_bytes.restype, L.mq_linear4_workspace_bytes.argtypes = sz, [pw, i64, i32, i32, i32]
         L.mq_linear4.restype, L.mq_linear4.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, vp, sz, vp]
-        L.mq_linear4_grad.restype, L.mq_linear4_grad.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, sz, vp]
-        L.mq_bias_grad_workspace_bytes.restype, L.mq_bias_grad_workspace_bytes.argtypes = sz, [i64, i64, i64]
-        L.mq_bias_grad.restype, L.mq_bias_grad.argtypes = ctypes.c_int, [vp, i32, i64, i64, i64, i64, vp, vp, vp, sz, vp]
+        L.mq_linear4_grad.restype, L.mq_linear4_grad.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, vp, sz, vp]
         _bound = L
     return _bound
 
@@ -257,57 +255,58 @@ def _rows_of(t):
     return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _product(t, weight, bias, counts, grad):
-    """One launch of mq_linear4 (grad: mq_linear4_grad) on rows t [R, K] ([R, N])."""
-    L = _bound or _bind()
-    rows = t.shape[0]
-    out = t.new_empty((rows, weight.k if grad else weight.n))
-    if not rows:
-        return out
-    t, ld = _rows_of(t)
+def _on_device(call, t, *args):
+    """call(t, *args) with t's device as the current one."""
     index = t.device.index
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return _launch(L, t, ld, rows, weight, bias, counts, grad, out, index)
-    return _launch(L, t, ld, rows, weight, bias, counts, grad, out, index)
+    if index == torch._C._cuda_getDevice():
+        return call(t, *args, index)
+    with torch.cuda.device(index):
+        return call(t, *args, index)
 
 
-def _launch(L, t, ld, rows, weight, bias, counts, grad, out, index):
-    x = t.data_ptr()
-    aligned = x % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 25 or rows == 1)
-    key = (rows, aligned, counts is not None, grad)
+def _workspace(weight, t, ld, counts, grad):
+    """-> (tensor | None, bytes).  Of this call alone: a captured graph keeps it in its own pool, and calls on other
+    streams have their own."""
+    rows = t.shape[0]
+    key = (rows, t.data_ptr() % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 25 or rows == 1), counts is not None, grad)
     need = weight._need.get(key)
     if need is None:
         if len(weight._need) >= 4096:
             weight._need.clear()
-        need = weight._need[key] = L.mq_linear4_workspace_bytes(weight._ref, *key)
-    # of this call alone: a captured graph keeps it in its own pool, and calls on other streams have their own
-    ws = torch.empty(need, dtype=torch.uint8, device=t.device) if need else None
-    wp = None if ws is None else ws.data_ptr()
-    cp = None if counts is None else counts.data_ptr()
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if grad:
-        rc = L.mq_linear4_grad(weight._ref, x, _XDTYPES[t.dtype], rows, ld, cp, out.data_ptr(), wp, need, stream)
-    else:
-        rc = L.mq_linear4(weight._ref, x, _XDTYPES[t.dtype], rows, ld, None if bias is None else bias.data_ptr(), cp,
-                          out.data_ptr(), wp, need, stream)
+        need = weight._need[key] = _bound.mq_linear4_workspace_bytes(weight._ref, *key)
+    return (torch.empty(need, dtype=torch.uint8, device=t.device) if need else None), need
+
+
+def _forward(x, weight, bias, counts, index):
+    L = _bound or _bind()
+    rows = x.shape[0]
+    y = x.new_empty((rows, weight.n))
+    if rows:
+        x, ld = _rows_of(x)
+        ws, need = _workspace(weight, x, ld, counts, 0)
+        rc = L.mq_linear4(weight._ref, x.data_ptr(), _XDTYPES[x.dtype], rows, ld, None if bias is None else bias.data_ptr(),
+                          None if counts is None else counts.data_ptr(), y.data_ptr(), None if ws is None else ws.data_ptr(),
+                          need, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            _lib.check(rc)
+    return y
+
+
+def _backward(dy, weight, counts, want_x, want_bias, index):
+    L = _bound or _bind()
+    rows, n = dy.shape
+    dx = dy.new_empty((rows, weight.k)) if want_x else None
+    db = dy.new_empty((n,) if weight.experts is None else (weight.experts, n)) if want_bias else None
+    if not rows:
+        return dx, None if db is None else db.zero_()
+    dy, ld = _rows_of(dy)
+    ws, need = _workspace(weight, dy, ld, counts, want_x + 2 * want_bias)
+    rc = L.mq_linear4_grad(weight._ref, dy.data_ptr(), _XDTYPES[dy.dtype], rows, ld, None if counts is None else counts.data_ptr(),
+                           None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(),
+                           None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc)
-    return out
-
-
-def _bias_grad(dy, experts, counts):
-    L = _bind()
-    rows, n = dy.shape
-    db = torch.empty((n,) if experts is None else (experts, n), dtype=dy.dtype, device=dy.device)
-    dy, ld = _rows_of(dy)
-    with torch.cuda.device(dy.device):
-        need = L.mq_bias_grad_workspace_bytes(rows, n, experts or 1)
-        ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
-        _lib.check(L.mq_bias_grad(dy.data_ptr() or None, _XDTYPES[dy.dtype], rows, n, ld, experts or 1,
-                                  None if counts is None else counts.data_ptr(), db.data_ptr(), ws.data_ptr(), need,
-                                  torch.cuda.current_stream().cuda_stream))
-    return db
+    return dx, db
 
 
 class _PackedProduct(torch.autograd.Function):
@@ -315,14 +314,14 @@ class _PackedProduct(torch.autograd.Function):
     def forward(ctx, x, bias, weight, counts):
         ctx.weight = weight
         ctx.save_for_backward(counts)
-        return _product(x, weight, bias, counts, False)
+        return _on_device(_forward, x, weight, bias, counts)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (counts,), weight = ctx.saved_tensors, ctx.weight
-        dx = _product(dy, weight, None, counts, True) if ctx.needs_input_grad[0] else None
-        db = _bias_grad(dy, weight.experts, counts) if ctx.needs_input_grad[1] else None
+        counts, = ctx.saved_tensors
+        want_x, want_bias = ctx.needs_input_grad[:2]
+        dx, db = _on_device(_backward, dy, ctx.weight, counts, want_x, want_bias)
         return dx, db, None, None
 
 
@@ -349,7 +348,7 @@ def _check_operands(x, weight, bias):
 def _run(x, weight, bias, counts):
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _PackedProduct.apply(x, bias, weight, counts)
-    return _product(x, weight, bias, counts, False)
+    return _on_device(_forward, x, weight, bias, counts)
 
 
 def packed_linear(x, weight: PackedWeight, bias=None):

@@ -122,6 +122,24 @@ def test_linear_backward(pk, fmt, bits, dtype):
             near(db, dy.double().sum(0), dy.double().abs().sum(0) * (m / 16 + 1), n, p, what=("db", n, k, g, m))
 
 
+def test_bias_gradient_over_many_rows(pk):
+    """Runs of rows whose sums a second launch adds; bias alone, without a gradient of x."""
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    p, *_ = weight(gen, (70, 64), "int4", 4, 32)
+    pe, *_ = weight(gen, (3, 70, 64), "int4", 4, 32)
+    for m in (512, 513, 1000, 5000):
+        x = torch.randn(m, 64, generator=gen, device="cuda").bfloat16()
+        dy = torch.randn(m, 70, generator=gen, device="cuda").bfloat16()
+        b = torch.zeros(70, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        db, = torch.autograd.grad(pk.packed_linear(x, p, b), b, dy)
+        near(db, dy.double().sum(0), dy.double().abs().sum(0) * (m / 16 + 1), 70, p, what=m)
+        be = torch.zeros(3, 70, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        c = torch.tensor([m // 2, 0, m - m // 2 - 7])
+        db, = torch.autograd.grad(pk.packed_expert_linear(x, pe, c.cuda(), be), be, dy)
+        for i, lo, hi in spans(c, m):
+            near(db[i], dy[lo:hi].double().sum(0), dy[lo:hi].double().abs().sum(0) * (m / 16 + 1), 70, pe, what=(m, i))
+
+
 def counts_of(kind, e, rows):
     c = torch.zeros(e, dtype=torch.int64)
     if kind == "even":

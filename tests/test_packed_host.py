@@ -61,14 +61,18 @@ def test_library_refuses_before_any_launch():
     assert call(bad) == _lib.ERR_UNSUPPORTED
     need = L.mq_linear4_workspace_bytes(ref(_c()), 4, 1, 0, 1)     # the gradient's turned operand
     assert need >= 16 * 1024
-    assert L.mq_linear4_grad(ref(_c()), 4096, _lib.F16, 4, 64, None, 4096, None, 0, None) == _lib.ERR_WORKSPACE
-    assert L.mq_linear4_grad(ref(_c()), 4096, _lib.F16, 4, 64, None, 4096, 4096, need - 1, None) == _lib.ERR_WORKSPACE
+    back = lambda dx, db, ws, size, c=_c(), dt=_lib.F16: L.mq_linear4_grad(ref(c), 4096, dt, 4, 64, None, dx, db, ws, size, None)
+    assert back(4096, None, None, 0) == _lib.ERR_WORKSPACE
+    assert back(4096, None, 4096, need - 1) == _lib.ERR_WORKSPACE
+    assert back(None, None, 4096, big) == _lib.ERR_ARG
+    assert back(None, 4097, 4096, big) == _lib.ERR_ALIGN
+    assert back(None, 4096, 4096, big, dt=_lib.F32) == _lib.ERR_UNSUPPORTED
+    assert back(None, 4096, 4096, big, c=_c(experts=3)) == _lib.ERR_ARG
+    assert L.mq_linear4_workspace_bytes(ref(_c()), 4, 1, 0, 2) == 0
+    assert L.mq_linear4_workspace_bytes(ref(_c()), 4096, 1, 0, 2) > 0      # runs of rows, added by a second launch
     assert L.mq_w4_pack(ref(_c()), None, 4096, None, None) == _lib.ERR_ARG
     assert L.mq_w4_pack(ref(_c()), 4096, 4096, 4096, None) == _lib.ERR_ARG         # a zero point with symmetric codes
     assert L.mq_w4_unpack(ref(_c()), None, None) == _lib.ERR_ARG
-    assert L.mq_bias_grad(4096, _lib.F16, 4, 64, 64, 1, None, 4096, None, 0, None) == _lib.ERR_WORKSPACE
-    assert L.mq_bias_grad(4096, _lib.F32, 4, 64, 64, 1, None, 4096, 4096, big, None) == _lib.ERR_UNSUPPORTED
-    assert L.mq_bias_grad(4096, _lib.F16, 4, 64, 64, 3, None, 4096, 4096, big, None) == _lib.ERR_ARG
 
 
 def test_pack_codes_refuses_what_does_not_belong_together():
