@@ -375,19 +375,31 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
     while (pl.waves > 1 && pl.waves * p->splits > p->rb) pl.waves /= 2;
     return pl;
   }
-  // Tiles of 128 rows where they occupy most compute units, 64 elsewhere (5632 x 2048, 256 rows: 24.7 against 17.6;
-  // 14336 x 4096, 256 rows: 47 against 51).  The gradient's 128 x 256 decodes half as often per product, which is what
-  // bounds it (4096 x 4096, 4096 rows: 162 against 235 with 128 x 128).
-  const int bn = grad ? 256 : 128;
-  pl.bm = (per + 127) / 128 * busy * ((p->ct * 16 + bn - 1) / bn) < (grad ? 64 : 192) ? 64 : 128;
-  pl.bn = pl.bm == 64 ? 128 : bn;
-  p->nblocks = (p->ct * 16 + pl.bn - 1) / pl.bn;
+  // Tile height and cuts of the contraction (pieces of at least 4 blocks of 128, joined by a second launch): the cheapest
+  // by what was measured on 4096 x 4096, microseconds per block of 128 for a compute unit with one tile and with two.
+  // 64 x 128: 0.9 and 1.55 (gradient 1.9 and 2.8), 128 x 128: 1.3 and 2.3, the gradient's 128 x 256: 3.4 and 5.0 (it
+  // decodes half as often per product, which is what bounds it: 4096 rows 162 against 235 with 128 x 128).  A join takes
+  // 3 and moves its sums at about 4 MB per microsecond.
+  static const double kTime[2][2][2] = {{{0.9, 1.55}, {1.3, 2.3}}, {{1.9, 2.8}, {3.4, 5.0}}};
+  double best = 0;
+  for (int tall = 0; tall < 2; ++tall) {
+    const int bm = tall ? 128 : 64, bn = tall && grad ? 256 : 128;
+    const int64_t nblocks = (p->ct * 16 + bn - 1) / bn;
+    // (the last tile of an expert is half full on average)
+    const int64_t tiles = (counted ? rows / bm + (busy + 1) / 2 : (rows + bm - 1) / bm) * nblocks;
+    for (int s = 1; s <= 8 && (s == 1 || p->rb >= 4 * s); s *= 2) {
+      const int64_t each = (tiles * s + 255) / 256;  // tiles of a compute unit
+      const double t = (each / 2 * kTime[grad][tall][1] + each % 2 * kTime[grad][tall][0]) * p->rb / s +
+                       (s > 1 ? 3 + 8e-6 * s * rows * p->ct * 16 / 4 : 0);
+      if (pl.bm && t >= best) continue;
+      best = t;
+      pl.bm = bm;
+      pl.bn = bn;
+      p->splits = s;
+      p->nblocks = (int32_t)nblocks;
+    }
+  }
   p->mblocks = (int32_t)row_blocks(pl.bm);
-  // Few tiles: the contraction is cut and the pieces joined, at least 4 blocks of 128 to a piece.  The gradient's tiles
-  // take a wave per SIMD each and want two (14336 x 4096, 2048 rows, 256 tiles: 368 against 282).
-  const int64_t tiles = (per + pl.bm - 1) / pl.bm * busy * p->nblocks;
-  const int most = grad && pl.bm == 128 ? 4 : 8;
-  while (p->splits < most && tiles * p->splits <= (grad ? 256 : 128) && p->rb >= 8 * p->splits) p->splits *= 2;
   return pl;
 }
 

@@ -278,11 +278,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
   __shared__ f32x4 lds_xs[XS ? 2 : 1][XS ? W * BM / 4 : 1];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
   const int wm = w % WM, wn = w / WM;
-  const int64_t mb = blockIdx.x % p.mblocks;
-  const int64_t tile0 = ((int64_t)(blockIdx.x / p.mblocks) * WN + wn) * NT;  // tiles of 32 columns
+  // Workgroups go to the eight chiplets in turn: row tile 8 i + c belongs to chiplet c, whose L2 then holds its rows for all
+  // columns; the row tiles behind the last eight are dealt out by columns.
+  const uint32_t whole = (uint32_t)p.mblocks / 8 * (uint32_t)p.nblocks * 8, id = blockIdx.x;
+  const uint32_t rows8 = id < whole ? (uint32_t)p.mblocks / 8 : (uint32_t)p.mblocks % 8;
+  const uint32_t at = id < whole ? id / 8 : id - whole;
+  const int mb = (int)(id < whole ? at % rows8 * 8 + id % 8 : (uint32_t)p.mblocks / 8 * 8 + at % rows8);
+  const int64_t tile0 = ((int64_t)(at / rows8) * WN + wn) * NT;  // tiles of 32 columns
   int expert, rows;
   int64_t row0;
-  if (!w4_find_tile(a, BM, (int)mb, expert, row0, rows)) return;
+  if (!w4_find_tile(a, BM, mb, expert, row0, rows)) return;
   f32x16 acc[MT][NT];     // GRAD: the matrix instructions' own sums
   float sum[MT][NT][16];  // forward: the scaled sums (single registers: they are never a matrix operand)
 #pragma unroll
