@@ -660,7 +660,7 @@ int mq_w4_pack(const mq_w4* w, const void* codes, const void* scale, const void*
 /* deq float16 [experts][n][k] = h(h(q - zero) * scale): the bits that the quantizers' own deq output has. */
 int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream);
 
-/* May be 0.  aligned: every row of x (dy) starts on a multiple of 16 bytes and the next one at most 2^25 elements on;
+/* May be 0.  aligned: every row of x (dy) starts on a multiple of 16 bytes and the next one at most 2^23 elements on;
  * other rows are copied first.
  * counted: counts will be given; grad: 0 for mq_linear4, for mq_linear4_grad 1 (dx), 2 (db) or 3 (both). */
 size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t aligned, int32_t counted, int32_t grad);

@@ -281,7 +281,7 @@ template <class T> __global__ __launch_bounds__(256) void k_w4_bias_join(const B
 namespace {
 
 constexpr int64_t kMaxK = 1 << 20, kMaxN = 1 << 22, kMaxExperts = 4096, kMaxRows = (int64_t)1 << 29;
-constexpr int64_t kMaxStride = 1 << 25;  // elements between rows that the kernels address in 32 bits
+constexpr int64_t kMaxStride = 1 << 23;  // elements between rows that the kernels address in 32 bits
 
 uint8_t e4m3_of(float v, bool* ok) {  // exact, or *ok = false
   for (int b = 0; b < 256; ++b) {

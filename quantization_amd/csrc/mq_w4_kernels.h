@@ -266,17 +266,23 @@ template <int NT, int W> struct W4Ahead {  // what a wave holds of a block that 
   uint32_t s[NT][W];
 };
 typedef __attribute__((address_space(1))) const void w4_global_t;
+#ifdef __HIP_DEVICE_COMPILE__
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_buffer(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);  // raw 32-bit data
+}
+#endif
 typedef __attribute__((address_space(3))) void w4_lds_t;
 
 template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int FS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, const W4Product p) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass has no buffer descriptors; it needs the kernel's name only)
   constexpr int BM = 32 * MT * WM, NW = WM * WN, CH = BM / 4 / NW;  // 1 KiB pieces (4 rows) per wave
   constexpr int W = 4 / FS;                                         // windows of a block with a scale each
   constexpr bool XS = KIND == W4_U4 && !GRAD;
   static_assert(BM / 4 % NW == 0 && BM % 64 == 0, "the rows of a block are dealt evenly");
   __shared__ u32x4 lds[2][BM * 16];
   __shared__ f32x4 lds_xs[XS ? 2 : 1][XS ? W * BM / 4 : 1];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int wm = w % WM, wn = w / WM;
   // Workgroups go to the eight chiplets in turn: row tile 8 i + c belongs to chiplet c, whose L2 then holds its rows for all
   // columns; the row tiles behind the last eight are dealt out by columns.
@@ -301,20 +307,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
 
   if (expert >= 0) {
     // 16-row tile of this lane's row: tiles past the end repeat the last one (their results are not stored)
-    const uint32_t* bp[NT];
+    // The loads go through buffer descriptors: one offset per lane for the whole loop, the block's in a scalar register.
+    const int64_t bt0 = (tile0 - wn * NT) * 2 < p.ct ? (tile0 - wn * NT) * 2 : p.ct - 1;  // the workgroup's first 16-row tile
+    const auto bsrc = w4_buffer(p.b + ((int64_t)expert * p.ct + bt0) * p.rb * 256, (uint32_t)(WN * NT * 2) * (uint32_t)p.rb * 1024u);
+    const auto xsrc = w4_buffer(p.x + row0 * p.ldx, (uint32_t)(((int64_t)(rows - 1) * p.ldx + (int64_t)p.rb * 128) * 2));
+    uint32_t bo[NT];
     int64_t pt[NT];  // forward: this lane's column in the parameters of group 0
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       int64_t t = (tile0 + n) * 2 + (l32 >> 4);
-      t = (int64_t)expert * p.ct + (t < p.ct ? t : p.ct - 1);
-      bp[n] = p.b + t * p.rb * 256 + (half * 16 + (lane & 15)) * 4;
-      pt[n] = t * a.gp * 16 + (lane & 15);
+      t = t < p.ct ? t : p.ct - 1;
+      bo[n] = (uint32_t)(t - bt0) * (uint32_t)p.rb * 1024u + (half * 16 + (lane & 15)) * 16;
+      pt[n] = ((int64_t)expert * p.ct + t) * a.gp * 16 + (lane & 15);
     }
-    const uint16_t* xp[CH];
+    uint32_t xo[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int r = (w * CH + c) * 4 + (lane >> 4);
-      xp[c] = p.x + (row0 + (r < rows ? r : rows - 1)) * p.ldx + (((lane & 15) ^ (r & 15)) * 8);
+      xo[c] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.ldx * 2u + (((lane & 15) ^ (r & 15)) * 16);
     }
     const int kb0 = (int)((int64_t)p.rb * blockIdx.y / p.splits), kb1 = (int)((int64_t)p.rb * (blockIdx.y + 1) / p.splits);
     int64_t st0[NT];  // gradient: this lane's first scale under column tile n
@@ -327,7 +337,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
     auto fetch = [&](int kb, int buf, W4Ahead<NT, GRAD ? 1 : W>& to) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        __builtin_amdgcn_global_load_lds((w4_global_t*)(xp[c] + (int64_t)kb * 128), (w4_lds_t*)&lds[buf][(w * CH + c) * 64], 16, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xsrc, (w4_lds_t*)&lds[buf][(w * CH + c) * 64], 16, xo[c], kb * 256, 0, 0);
       if constexpr (XS) {  // 64 row sums to a wave's load; a tile may read past the last row
 #pragma unroll
         for (int c = 0; c < W * BM / 64; ++c)
@@ -338,7 +348,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) to.b[n][h] = *reinterpret_cast<const u32x4*>(bp[n] + (int64_t)kb * 256 + h * 128);
+        for (int h = 0; h < 2; ++h) to.b[n][h] = __builtin_amdgcn_raw_buffer_load_b128(bsrc, bo[n] + h * 512, kb * 1024, 0);
         if constexpr (!GRAD) {
 #pragma unroll
           for (int v = 0; v < W; ++v) {
@@ -384,6 +394,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               s[n] = (float)h_from_bits(cur.s[n][v]);
+              asm("" : "+v"(s[n]));  // a float32 register: v_fmac_f32 issues faster than the mixed fma the compiler would choose
               if constexpr (KIND == W4_U4) sz[n] = -(s[n] * (float)h_from_bits(cur.s[n][v] >> 16));  // exact: 11 x 11 bits
             }
 #pragma unroll
@@ -472,6 +483,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
         }
       }
   }
+#endif
 }
 
 // Sums of x over the windows of 32 FS columns that k_w4_gemm scales at a time: xs[window][row], for the zero points.

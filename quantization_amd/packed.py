@@ -268,7 +268,7 @@ def _workspace(weight, t, ld, counts, grad):
     """-> (tensor | None, bytes).  Of this call alone: a captured graph keeps it in its own pool, and calls on other
     streams have their own."""
     rows = t.shape[0]
-    key = (rows, t.data_ptr() % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 25 or rows == 1), counts is not None, grad)
+    key = (rows, t.data_ptr() % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 23 or rows == 1), counts is not None, grad)
     need = weight._need.get(key)
     if need is None:
         if len(weight._need) >= 4096:
