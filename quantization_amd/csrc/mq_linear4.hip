@@ -103,7 +103,7 @@ template <int KIND> __global__ __launch_bounds__(256) void k_w4_unpack(const W4A
     s = (float)h_from_bits(static_cast<const uint16_t*>(a.params)[at]);
   }
   for (int i = 0; i < 8 && k0 + i < a.k; ++i) {
-    float q = f[i] * w4_f32_scale<KIND>();
+    float q = f[i];
     if constexpr (KIND == W4_U4) q = (float)h_from_bits(f2h_bits(q - z));
     out[(e * a.n + n) * a.k + k0 + i] = (uint16_t)f2h_bits(q * s);
   }
@@ -197,7 +197,7 @@ template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args
     }
   }
   // scales of the groups that begin in this block of columns
-  const float up = t.half ? a.norm[e] : w4_f32_scale<KIND>();
+  const float up = t.half ? a.norm[e] : 1.0f;
   for (int j = 0; j < 4; ++j) {
     const int step = blockIdx.x * 4 + j, grp = w4_group(a, step);
     if (grp * a.gu != step || grp >= a.gp) continue;
@@ -215,12 +215,12 @@ template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args
         }
       }
       const int64_t to = (e * a.gp + grp) * t.rb * 128 + n;
-      if (t.half) {
-        static_cast<uint16_t*>(t.ts)[to] = W4F16::from_f32(s * up);
-        if constexpr (KIND == W4_U4) static_cast<uint16_t*>(t.tz)[to] = W4F16::from_f32(z);
-      } else {
-        static_cast<float*>(t.ts)[to] = s * up;
-        if constexpr (KIND == W4_U4) static_cast<float*>(t.tz)[to] = s * z;  // exact: 11 x 11 bits
+      static_cast<uint16_t*>(t.ts)[to] = W4F16::from_f32(s * up);
+      if constexpr (KIND == W4_U4) {
+        if (t.half)
+          static_cast<uint16_t*>(t.tz)[to] = W4F16::from_f32(z);
+        else
+          static_cast<float*>(t.tz)[to] = s * z;  // exact: 11 x 11 bits
       }
     }
   }
@@ -270,17 +270,18 @@ template <class T> __global__ __launch_bounds__(1024) void k_w4_bias(const BiasA
   }
 }
 template <class T> __global__ __launch_bounds__(256) void k_w4_bias_join(const BiasArgs p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = p.experts * p.n;
-  if (i >= total) return;
-  float s = p.part[i];
-  for (int o = 1; o < p.splits; ++o) s += p.part[o * total + i];
-  p.db[i] = T::from_f32(s);
+  const int64_t total = p.experts * p.n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float s = p.part[i];
+    for (int o = 1; o < p.splits; ++o) s += p.part[o * total + i];
+    p.db[i] = T::from_f32(s);
+  }
 }
 
 // ---- host side -----------------------------------------------------------------------------------------
 namespace {
 
-constexpr int64_t kMaxK = 1 << 20, kMaxN = 1 << 22, kMaxExperts = 4096, kMaxRows = (int64_t)1 << 29;
+constexpr int64_t kMaxK = 1 << 20, kMaxN = 1 << 22, kMaxExperts = 4096, kMaxRows = (int64_t)1 << 27;
 constexpr int64_t kMaxStride = 1 << 23;  // elements between rows that the kernels address in 32 bits
 
 uint8_t e4m3_of(float v, bool* ok) {  // exact, or *ok = false
@@ -303,6 +304,7 @@ int check_w4(const mq_w4* w) {
   if (w->group < 0) return MQ_ERR_ARG;
   if (w->group > 0 && w->k % w->group) return MQ_ERR_GROUP;
   if (w->group > 0 && w->group % 32) return MQ_ERR_UNSUPPORTED;
+  if (w->kind == W4_LUT && w->values[0] != 0.0f) return MQ_ERR_UNSUPPORTED;  // (padding is code 0)
   return MQ_OK;
 }
 int32_t steps_of_group(const mq_w4* w) { return (int32_t)(w->group > 0 ? w->group / 32 : w4_ktiles(w->k) * 4); }
@@ -427,8 +429,8 @@ size_t bias_bytes(const mq_w4* w, int64_t rows) {
 }
 template <class T> hipError_t bias_launch(const BiasArgs& p, hipStream_t st) {
   hipLaunchKernelGGL((k_w4_bias<T>), dim3((unsigned)((p.n + 63) / 64), p.splits, (unsigned)p.experts), dim3(1024), 0, st, p);
-  if (p.part)
-    hipLaunchKernelGGL((k_w4_bias_join<T>), dim3((unsigned)((p.experts * p.n + 255) / 256)), dim3(256), 0, st, p);
+  const int64_t join = (p.experts * p.n + 255) / 256;
+  if (p.part) hipLaunchKernelGGL((k_w4_bias_join<T>), dim3((unsigned)(join < 4096 ? join : 4096)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
@@ -448,7 +450,8 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   if (rc != MQ_OK) return rc;
   W4Product p = {};
   const W4Plan pl = plan_of(w, rows, grad, counts != nullptr, &p);
-  if ((int64_t)p.nblocks * p.mblocks > (int64_t)0x7FFFFFFF) return MQ_ERR_TOO_LARGE;
+  // (a launch counts its threads in 32 bits)
+  if ((int64_t)p.nblocks * p.mblocks * (pl.bm ? 256 : 64 * pl.waves) >= (int64_t)1 << 32) return MQ_ERR_TOO_LARGE;
   p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
   // workspace: the turned operand (gradient) or the row sums, the splits' partial sums, the padded rows
   const size_t sums = sums_bytes(w, pl, p, rows, grad), turned = grad ? turn_bytes(w) : sums;

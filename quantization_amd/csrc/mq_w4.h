@@ -149,8 +149,7 @@ template <class T, int KIND> __device__ __forceinline__ u32x4 w4_decode(uint32_t
   }
   return r;
 }
-// Dword -> its eight codes' values in float32, divided by w4_f32_scale<KIND>().
-template <int KIND> constexpr float w4_f32_scale() { return KIND == W4_FP4 ? 1.0f : w4_byte_scale<KIND>(); }
+// Dword -> its eight codes' values in float32.
 template <int KIND> __device__ __forceinline__ void w4_decode_f32(uint32_t d, const W4Lut& lut, float* f) {
   w4_f2 p[4];
   if constexpr (KIND == W4_FP4) {
@@ -161,10 +160,11 @@ template <int KIND> __device__ __forceinline__ void w4_decode_f32(uint32_t d, co
   } else {
     uint32_t lo, hi;
     w4_bytes<KIND>(d, lut, lo, hi);
-    p[0] = __builtin_amdgcn_cvt_pk_f32_fp8(lo, false);
-    p[1] = __builtin_amdgcn_cvt_pk_f32_fp8(lo, true);
-    p[2] = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false);
-    p[3] = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+    constexpr float s = w4_byte_scale<KIND>();
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, s, false);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, s, true);
+    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, s, false);
+    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, s, true);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[2 * i] = p[i][0], f[2 * i + 1] = p[i][1];

@@ -227,10 +227,10 @@ template <int KIND> struct W4Scales<W4F16, KIND> {
   }
 };
 template <int KIND> struct W4Scales<W4BF16, KIND> {
-  f32x4 s[2], z[2];
+  u32x4 s;     // float16 as they are: v_fma_mix_f32 takes them so, and half the bytes come through the cache
+  f32x4 z[2];  // scale * zero
   __device__ __forceinline__ void load(const W4Product& p, int64_t at) {
-    const f32x4* from = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.ts) + at);
-    s[0] = from[0], s[1] = from[1];
+    s = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.ts) + at);
     if constexpr (KIND == W4_U4) {
       const f32x4* zero = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.tz) + at);
       z[0] = zero[0], z[1] = zero[1];
@@ -239,9 +239,9 @@ template <int KIND> struct W4Scales<W4BF16, KIND> {
   __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
     float f[8];
     w4_decode_f32<KIND>(d, lut, f);
+    const w4_h8 h = __builtin_bit_cast(w4_h8, s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      f[i] = KIND == W4_U4 ? __builtin_fmaf(f[i], s[i / 4][i % 4], -z[i / 4][i % 4]) : f[i] * s[i / 4][i % 4];
+    for (int i = 0; i < 8; ++i) f[i] = __builtin_fmaf(f[i], (float)h[i], KIND == W4_U4 ? -z[i / 4][i % 4] : 0.0f);
     u32x4 v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = W4BF16::pack(f[2 * i], f[2 * i + 1]);

@@ -98,6 +98,7 @@ class PackedWeight:
     of dtype touches them.  experts: E, or None for a single weight."""
 
     def __init__(self, data, params, norm, experts, n, k, group_size, wq_bits, datatype):
+        """Takes the three tensors as they are; their sizes have to be what pack_codes made for this weight."""
         self.data, self.params, self.norm = data, params, norm
         self.experts, self.n, self.k = experts, int(n), int(k)
         self.group_size, self.wq_bits, self.datatype = _group(group_size), wq_bits, datatype
@@ -105,10 +106,17 @@ class PackedWeight:
 
     def _describe(self):
         kind, values = _kind_of(self.wq_bits, self.datatype)
+        L = _bind()
         s = _W4(data=self.data.data_ptr() or None, params=self.params.data_ptr() or None, norm=self.norm.data_ptr() or None,
                 experts=self.experts or 1, n=self.n, k=self.k, group=max(self.group_size, 0), kind=kind)
         if values is not None:
             s.values[:] = values
+        for t, dtype, nbytes in ((self.data, torch.int32, L.mq_w4_data_bytes(self.experts or 1, self.n, self.k)),
+                                 (self.params, torch.int16, L.mq_w4_params_bytes(ctypes.byref(s))),
+                                 (self.norm, torch.int32, 4 * (self.experts or 1))):
+            if t.dtype != dtype or t.numel() * t.element_size() != nbytes or not nbytes or not t.is_contiguous() \
+                    or t.device != self.data.device:
+                raise ValueError(f"not the tensors of a packed weight: {t.dtype} {tuple(t.shape)} on {t.device}")
         self._c = s
         self._ref = ctypes.byref(s)
         self._need = {}   # workspace bytes by (rows, aligned, counted, grad)
@@ -388,18 +396,20 @@ class PackedLinear(nn.Module):
     def __init__(self, src: nn.Linear, wq_bits: int = 4, datatype: str = "int4", group_size=None):
         super().__init__()
         self.in_features, self.out_features = src.in_features, src.out_features
-        self.packed = pack_weight(src.weight.data, wq_bits, datatype, group_size)
+        self._packed = pack_weight(src.weight.data, wq_bits, datatype, group_size)
         for name in ("data", "params", "norm"):
-            self.register_buffer("weight_" + name, getattr(self.packed, name))
-        self.bias = None if src.bias is None else nn.Parameter(src.bias.detach().to(self.packed.device),
+            self.register_buffer("weight_" + name, getattr(self._packed, name))
+        self.bias = None if src.bias is None else nn.Parameter(src.bias.detach().to(self._packed.device),
                                                                requires_grad=src.bias.requires_grad)
 
-    def _apply(self, fn, recurse=True):
-        super()._apply(fn, recurse)   # buffers may have moved: the description holds their addresses
-        p = self.packed
-        self.packed = PackedWeight(self.weight_data, self.weight_params, self.weight_norm, p.experts, p.n, p.k, p.group_size,
-                                   p.wq_bits, p.datatype)
-        return self
+    @property
+    def packed(self) -> PackedWeight:
+        """The weight that the buffers hold (moved, loaded or assigned ones are taken up)."""
+        p = self._packed
+        if p.data is not self.weight_data or p.params is not self.weight_params or p.norm is not self.weight_norm:
+            p = self._packed = PackedWeight(self.weight_data, self.weight_params, self.weight_norm, p.experts, p.n, p.k,
+                                            p.group_size, p.wq_bits, p.datatype)
+        return p
 
     def forward(self, x):
         return packed_linear(x, self.packed, self.bias)

@@ -356,6 +356,42 @@ def test_streams_and_graphs(pk):
             assert torch.equal(a, e), i
 
 
+def test_offsets_beyond_32_bits(pk):
+    """Rows of x, of y and tiles of the weight that lie more than 2^32 bytes from the first."""
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    n, k = 64, 256
+    p, w, mass, _ = weight(gen, (n, k), "int4_asym", 4, 64)
+    for stride, rows in ((1 << 23, 300), ((1 << 23) + 8, 300), (1 << 28, 9)):     # read in place, copied first, few rows
+        x = torch.empty((rows - 1) * stride + k, dtype=torch.float16, device="cuda").as_strided((rows, k), (stride, 1))
+        x.copy_(torch.randn(rows, k, generator=gen, device="cuda"))
+        near(pk.packed_linear(x, p), product(x, w), product(x.abs(), mass), k, p, what=stride)
+        del x
+    n, k, rows = 16400, 32, 140000                                               # y: 4.6 GB, dy too
+    p, w, mass, _ = weight(gen, (n, k), "int4", 4, 32)
+    x = torch.randn(rows, k, generator=gen, device="cuda").half().requires_grad_()
+    y = pk.packed_linear(x, p)
+    dx, = torch.autograd.grad(y, x, y.detach())
+    with torch.no_grad():
+        at = torch.tensor([0, 1, 65535, 131000, 139935, 139999], device="cuda")
+        near(y[at], product(x[at], w), product(x[at].abs(), mass), k, p, what="y")
+        near(dx[at], product(y[at], w.t()), product(y[at].abs(), w.t().abs()), n, p, rounded=True, what="dx")
+    del x, y, dx
+    e, n, k = 40, 16384, 16384                                                   # 5.4 GB of codes
+    q = torch.randint(-7, 8, (e, n, k), generator=gen, device="cuda", dtype=torch.int8)
+    s = (torch.rand(e, n, 1, generator=gen, device="cuda") * 0.01).half()
+    p = pk.pack_codes(q, s[..., 0], None, 4, "int4", None)
+    counts = torch.zeros(e, dtype=torch.int32, device="cuda")
+    counts[-1], counts[0] = 50, 50
+    x = torch.randn(100, k, generator=gen, device="cuda").half().requires_grad_()
+    y = pk.packed_expert_linear(x, p, counts)
+    dx, = torch.autograd.grad(y, x, y.detach())
+    with torch.no_grad():
+        for i, lo in ((0, 0), (e - 1, 50)):
+            w = q[i].double() * s[i].double()
+            near(y[lo:lo + 50], product(x[lo:lo + 50], w), product(x[lo:lo + 50].abs(), w.abs()), k, p, what=i)
+            near(dx[lo:lo + 50], product(y[lo:lo + 50], w.t()), product(y[lo:lo + 50].abs(), w.t().abs()), n, p, rounded=True, what=i)
+
+
 def test_repeated_calls_have_the_same_bits(pk):
     gen = torch.Generator(device="cuda").manual_seed(13)
     p, *_ = weight(gen, (256, 2048), "fp4", 4, 64)
@@ -405,6 +441,11 @@ def test_quant_model_packed(pk, fmt, bits, g):
             t.zero_()
     again.load_state_dict(state)
     assert torch.equal(again(x), model(x))
+    other = copy.deepcopy(model)
+    for t in other.state_dict().values():
+        t.zero_()
+    other.load_state_dict(state, assign=True)
+    assert torch.equal(other(x), model(x))
     half = copy.deepcopy(model).bfloat16()     # the packed weight has no floating dtype to change
     assert half(x.bfloat16()).dtype == torch.bfloat16
 

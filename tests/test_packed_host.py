@@ -59,6 +59,9 @@ def test_library_refuses_before_any_launch():
     bad = _c(kind=packed.TABLE)
     bad.values[1] = 17.5                                        # not an e4m3 number
     assert call(bad) == _lib.ERR_UNSUPPORTED
+    bad.values[0], bad.values[1] = 1.0, 1.0
+    assert call(bad) == _lib.ERR_UNSUPPORTED                    # entry 0 is what padding decodes to
+    assert call(_c(n=1 << 22, k=1 << 20, group=0), rows=1 << 27, ld=1 << 20) in (_lib.ERR_TOO_LARGE, _lib.ERR_WORKSPACE)
     need = L.mq_linear4_workspace_bytes(ref(_c()), 4, 1, 0, 1)     # the gradient's turned operand
     assert need >= 16 * 1024
     back = lambda dx, db, ws, size, c=_c(), dt=_lib.F16: L.mq_linear4_grad(ref(c), 4096, dt, 4, 64, None, dx, db, ws, size, None)
