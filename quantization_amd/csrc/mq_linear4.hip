@@ -379,10 +379,10 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
   }
   // Tile height and cuts of the contraction (pieces of at least 4 blocks of 128, joined by a second launch): the cheapest
   // by what was measured on 4096 x 4096, microseconds per block of 128 for a compute unit with one tile and with two.
-  // 64 x 128: 0.9 and 1.55 (gradient 1.9 and 2.8), 128 x 128: 1.3 and 2.3, the gradient's 128 x 256: 3.4 and 5.0 (it
-  // decodes half as often per product, which is what bounds it: 4096 rows 162 against 235 with 128 x 128).  A join takes
-  // 3 and moves its sums at about 4 MB per microsecond.
-  static const double kTime[2][2][2] = {{{0.9, 1.55}, {1.3, 2.3}}, {{1.9, 2.8}, {3.4, 5.0}}};
+  // 64 x 128: 0.7 and 1.55 (gradient 1.5 and 2.9), 128 x 128: 1.3 and 2.3, the gradient's 128 x 256: 3.4 and 5.0 (it
+  // decodes half as often per product, which is what bounds it: 4096 rows 162 against 235 with 128 x 128).  A tile begins
+  // and ends in 1.5; a join takes 3 and moves its sums at about 4 MB per microsecond.
+  static const double kTime[2][2][2] = {{{0.7, 1.55}, {1.3, 2.3}}, {{1.5, 2.9}, {3.4, 5.0}}};
   double best = 0;
   for (int tall = 0; tall < 2; ++tall) {
     const int bm = tall ? 128 : 64, bn = tall && grad ? 256 : 128;
@@ -391,7 +391,7 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
     const int64_t tiles = (counted ? rows / bm + (busy + 1) / 2 : (rows + bm - 1) / bm) * nblocks;
     for (int s = 1; s <= 8 && (s == 1 || p->rb >= 4 * s); s *= 2) {
       const int64_t each = (tiles * s + 255) / 256;  // tiles of a compute unit
-      const double t = (each / 2 * kTime[grad][tall][1] + each % 2 * kTime[grad][tall][0]) * p->rb / s +
+      const double t = (each / 2 * kTime[grad][tall][1] + each % 2 * kTime[grad][tall][0]) * p->rb / s + 1.5 * each +
                        (s > 1 ? 3 + 8e-6 * s * rows * p->ct * 16 / 4 : 0);
       if (pl.bm && t >= best) continue;
       best = t;
@@ -451,7 +451,7 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   W4Product p = {};
   const W4Plan pl = plan_of(w, rows, grad, counts != nullptr, &p);
   // (a launch counts its threads in 32 bits)
-  if ((int64_t)p.nblocks * p.mblocks * (pl.bm ? 256 : 64 * pl.waves) >= (int64_t)1 << 32) return MQ_ERR_TOO_LARGE;
+  if ((int64_t)p.nblocks * p.mblocks * (pl.bm ? 512 : 64 * pl.waves) >= (int64_t)1 << 32) return MQ_ERR_TOO_LARGE;
   p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
   // workspace: the turned operand (gradient) or the row sums, the splits' partial sums, the padded rows
   const size_t sums = sums_bytes(w, pl, p, rows, grad), turned = grad ? turn_bytes(w) : sums;

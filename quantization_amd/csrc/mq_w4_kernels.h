@@ -257,6 +257,8 @@ template <int KIND> struct W4Scales<W4BF16, KIND> {
 // fetched in whole lines and neither the writes nor the operand reads meet in a bank.  The packed weight goes from memory
 // straight into the registers of the wave that decodes it: lane l takes row l % 32 of the 32-row tile, the halves of its
 // wave the eight columns 8 (l / 32) of every sixteen -- two of the layout's four dwords-quadruples.
+// WK = 2: two sets of waves with buffers of their own take the blocks of the contraction in turn, for small tiles, where
+// one wave per SIMD would wait for its own decoding.
 // Rows are 16-byte aligned and a multiple of 128 long here: others are copied first (k_w4_pad).
 // GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.
 // GRAD = true (dx = dy W, operand b transposed): scales change along the contraction, so they are multiplied into the
@@ -273,17 +275,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_buffer(const void* base, ui
 #endif
 typedef __attribute__((address_space(3))) void w4_lds_t;
 
-template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int FS>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, const W4Product p) {
+template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int WK, int FS>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a, const W4Product p) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass has no buffer descriptors; it needs the kernel's name only)
   constexpr int BM = 32 * MT * WM, NW = WM * WN, CH = BM / 4 / NW;  // 1 KiB pieces (4 rows) per wave
   constexpr int W = 4 / FS;                                         // windows of a block with a scale each
   constexpr bool XS = KIND == W4_U4 && !GRAD;
   static_assert(BM / 4 % NW == 0 && BM % 64 == 0, "the rows of a block are dealt evenly");
-  __shared__ u32x4 lds[2][BM * 16];
-  __shared__ f32x4 lds_xs[XS ? 2 : 1][XS ? W * BM / 4 : 1];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
-  const int wm = w % WM, wn = w / WM;
+  __shared__ u32x4 lds_all[WK][2][BM * 16];
+  __shared__ f32x4 lds_xs_all[WK][XS ? 2 : 1][XS ? W * BM / 4 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
+  const int w = wave % NW, wk = wave / NW, wm = w % WM, wn = w / WM;
+  auto& lds = lds_all[wk];
+  auto& lds_xs = lds_xs_all[wk];
   // Workgroups go to the eight chiplets in turn: row tile 8 i + c belongs to chiplet c, whose L2 then holds its rows for all
   // columns; the row tiles behind the last eight are dealt out by columns.
   const uint32_t whole = (uint32_t)p.mblocks / 8 * (uint32_t)p.nblocks * 8, id = blockIdx.x;
@@ -361,12 +365,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
         }
       }
     };
-    if (kb0 < kb1) fetch(kb0, 0, next);
+    if (kb0 + wk < kb1) fetch(kb0 + wk, 0, next);
     __syncthreads();
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const int buf = (kb - kb0) & 1;
+    for (int it = 0; kb0 + it * WK < kb1; ++it) {
+      const int kb = kb0 + it * WK + wk, buf = it & 1;
       const W4Ahead<NT, GRAD ? 1 : W> cur = next;
-      if (kb + 1 < kb1) fetch(kb + 1, buf ^ 1, next);
+      if (kb + WK < kb1) fetch(kb + WK, buf ^ 1, next);
       const u32x4* xb = lds[buf] + (wm * MT * 32 + l32) * 16;
       const int turn = (l32 & 15) ^ half;
       // One row tile: its operands of the whole block at once, since two products hide no LDS load.
@@ -375,7 +379,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
 #pragma unroll
         for (int st = 0; st < 8; ++st) xa[st] = xb[(2 * st) ^ turn];
       }
-      if constexpr (!GRAD) {
+      if (WK > 1 && kb >= kb1) {
+        // the other waves' last block: nothing for this half
+      } else if constexpr (!GRAD) {
         f32x16 tmp[MT][NT];
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
@@ -446,6 +452,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_w4_gemm(const W4Args a, con
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum[m][n][i] = acc[m][n][i] * down;
     }
+  }
+  if constexpr (WK > 1) {  // the halves' sums, through the buffers that nobody reads any more
+    float* red = reinterpret_cast<float*>(lds_all) + (w * MT * NT * 16) * 64 + lane;
+    static_assert(WK == 2 && sizeof(lds_all) >= NW * MT * NT * 16 * 64 * 4, "the sums of one half fit");
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (wk) red[((m * NT + n) * 16 + i) * 64] = sum[m][n][i];
+    __syncthreads();
+    if (wk) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[m][n][i] += red[((m * NT + n) * 16 + i) * 64];
   }
   // A lane holds one column; neighbours exchange half of their rows, so that each stores pairs of columns: the even lane
   // of a pair rows 0, 2, .. of its registers, the odd one rows 1, 3, ..
@@ -532,20 +557,20 @@ static void w4_rows_go(const W4Args& a, const W4Product& p, const W4Plan& pl, hi
   else
     hipLaunchKernelGGL((k_w4_rows<T, KIND, MT, NT, 1>), grid, block, lds, st, a, p);
 }
-template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN>
+template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int WK>
 static void w4_gemm_go(const W4Args& a, const W4Product& p, const W4Plan& pl, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)p.nblocks * p.mblocks), p.splits), block(64 * WM * WN);
+  const dim3 grid((unsigned)((int64_t)p.nblocks * p.mblocks), p.splits), block(64 * WM * WN * WK);
   const dim3 sums((unsigned)((a.rows + 15) / 16), p.rb);
   constexpr bool xs = KIND == W4_U4 && !GRAD;
   if (GRAD ? pl.fs >= 2 : pl.fs == 4) {
     if (xs) hipLaunchKernelGGL((k_w4_rowsum<T, 4>), sums, dim3(256), 0, st, p, a.rows, p.xs);
-    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, 4>), grid, block, 0, st, a, p);
+    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, WK, 4>), grid, block, 0, st, a, p);
   } else if (!GRAD && pl.fs == 2) {
     if (xs) hipLaunchKernelGGL((k_w4_rowsum<T, 2>), sums, dim3(256), 0, st, p, a.rows, p.xs);
-    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, GRAD ? 4 : 2>), grid, block, 0, st, a, p);
+    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, WK, GRAD ? 4 : 2>), grid, block, 0, st, a, p);
   } else {
     if (xs) hipLaunchKernelGGL((k_w4_rowsum<T, 1>), sums, dim3(256), 0, st, p, a.rows, p.xs);
-    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, 1>), grid, block, 0, st, a, p);
+    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, WK, 1>), grid, block, 0, st, a, p);
   }
 }
 
@@ -559,11 +584,11 @@ hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool
     else if (pl.nt == 2) w4_rows_go<T, KIND, 2, 2>(a, p, pl, st);
     else w4_rows_go<T, KIND, 2, 4>(a, p, pl, st);
   } else if (grad) {
-    if (pl.bm == 64) w4_gemm_go<T, KIND, true, 1, 2, 2, 2>(a, p, pl, st);
-    else w4_gemm_go<T, KIND, true, 4, 2, 1, 4>(a, p, pl, st);
+    if (pl.bm == 64) w4_gemm_go<T, KIND, true, 1, 2, 2, 2, 2>(a, p, pl, st);
+    else w4_gemm_go<T, KIND, true, 4, 2, 1, 4, 1>(a, p, pl, st);
   } else {
-    if (pl.bm == 64) w4_gemm_go<T, KIND, false, 1, 2, 2, 2>(a, p, pl, st);
-    else w4_gemm_go<T, KIND, false, 2, 2, 2, 2>(a, p, pl, st);
+    if (pl.bm == 64) w4_gemm_go<T, KIND, false, 1, 2, 2, 2, 2>(a, p, pl, st);
+    else w4_gemm_go<T, KIND, false, 2, 2, 2, 2, 1>(a, p, pl, st);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.part) return e;
