@@ -622,8 +622,8 @@ int mq_histogram(const void* x, int32_t dtype, int64_t n, const double* edges, i
  *
  * x, dy, bias: float16 or bfloat16, y / dx of the same type, sums in float32, one rounding at the end.  In mq_linear4
  * the codes' values enter the matrix cores exactly and the scales are applied in float32.  In mq_linear4_grad the scales
- * change along the sum, so each weight is rounded once to the type of dy (half a step: 2^-12 of it in float16, 2^-9 in
- * bfloat16).  With zero points the sum is taken as scale * sum(q x) - scale * zero * sum(x): an infinite x[r][k] makes
+ * change along the sum, so each weight is rounded once to float16 (by 2^-11 of it at most); rows of bfloat16 are brought
+ * into float16's range by a power of two each, exactly but for values more than 2^28 below their row's largest.  With zero points the sum is taken as scale * sum(q x) - scale * zero * sum(x): an infinite x[r][k] makes
  * the whole row NaN where (q - zero) x would have left infinities.
  *
  * Rows and experts: counts == NULL: one weight (experts == 1) for all rows.  Otherwise the rows are sorted by expert and
@@ -663,7 +663,8 @@ int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream);
 /* May be 0.  aligned: every row of x (dy) starts on a multiple of 16 bytes and the next one at most 2^23 elements on;
  * other rows are copied first.
  * counted: counts will be given; grad: 0 for mq_linear4, for mq_linear4_grad 1 (dx), 2 (db) or 3 (both). */
-size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t aligned, int32_t counted, int32_t grad);
+size_t mq_linear4_workspace_bytes(const mq_w4* w, int32_t dtype, int64_t rows, int32_t aligned, int32_t counted,
+                                  int32_t grad);
 /* x [rows][ldx] (ldx elements from row to row, 0 = the same row again), y [rows][n] contiguous, 16-byte aligned. */
 int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
                const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream);

@@ -116,6 +116,43 @@ __global__ __launch_bounds__(256) void k_w4_pad(const W4Product p, int64_t rows,
   if (r < rows) *reinterpret_cast<u32x4*>(to + r * p.rb * 128 + k) = w4_load8(p.x + r * p.ldx, k, p.kc, p.vec);
 }
 
+// Rows of bfloat16 -> rows of float16 times a power of two each, which brings a row's largest value into [2^14, 2^15):
+// eight significant bits fit float16's eleven, so nothing is lost but of values more than 2^28 below the largest.
+// down[row]: the inverse factor.  A row that holds an infinity or NaN keeps its scale (its results are not finite anyway).
+// One wave to a row; the second pass finds the row in the caches.
+__device__ __forceinline__ void w4_half_row(const W4Product& p, int64_t row, uint16_t* to, float* down) {
+  const int lane = threadIdx.x & 63;
+  const uint16_t* from = p.x + row * p.ldx;
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int64_t k = lane * 8; k < p.kc; k += 512) {
+    const u32x4 v = w4_load8(from, k, p.kc, p.vec);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = v[i] & 0x7FFFu, hi = v[i] >> 16 & 0x7FFFu;
+      m = m > lo ? m : lo;
+      m = m > hi ? m : hi;
+    }
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
+    m = m > o ? m : o;
+  }
+  const int e = (int)(m >> 7);
+  int shift = e == 255 ? 0 : 141 - (e ? e : 1);
+  if (shift > 126) shift = 126;
+  const float up = f_from_bits((uint32_t)(127 + shift) << 23);
+  if (lane == 0) down[row] = f_from_bits((uint32_t)(127 - shift) << 23);
+#pragma unroll 4
+  for (int64_t k = lane * 8; k < (int64_t)p.rb * 128; k += 512) {
+    u32x4 v = w4_load8(from, k, p.kc, p.vec);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = W4F16::pack(f_from_bits(v[i] << 16) * up, f_from_bits(v[i] & 0xFFFF0000u) * up);
+    *reinterpret_cast<u32x4*>(to + row * p.rb * 128 + k) = v;
+  }
+}
+
 // ---- the transposed operand of the gradient ----------------------------------------------------------
 // dx = dy W contracts over the weight's rows: the same codes in the same layout with the roles of rows and columns
 // exchanged.  A wave turns 128 rows x 128 columns, a thread 8 rows x 32 columns: it
@@ -125,9 +162,12 @@ __global__ __launch_bounds__(256) void k_w4_pad(const W4Product p, int64_t rows,
 // It also writes the scales (and zero points) along the contraction, in the form that W4Scales loads.
 struct TurnArgs {
   uint32_t* out;  // [E][ct][rb][64][4]
-  void* ts;       // [E][GP][128 rb]
-  void* tz;
-  int32_t ct, rb, half;
+  uint16_t* ts;   // [E][GP][128 rb]
+  uint16_t* tz;
+  int32_t ct, rb;
+  uint32_t blocks;   // workgroups that turn; the others bring rows of bfloat16 to float16
+  uint16_t* half;
+  float* down;
 };
 // Nibble r of b[c] = nibble c of a[r].
 __device__ __forceinline__ void w4_turn8(uint32_t* a) {
@@ -151,18 +191,23 @@ __device__ __forceinline__ void w4_turn8(uint32_t* a) {
     a[r + 4] = __builtin_amdgcn_perm(y, x, 0x07060302u);
   }
 }
-template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args a, const TurnArgs t) {
+template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args a, const TurnArgs t, const W4Product p) {
   __shared__ u32x4 lds[512];
+  if (blockIdx.x >= t.blocks) {
+    for (int64_t row = blockIdx.x - t.blocks; row < a.rows; row += gridDim.x - t.blocks) w4_half_row(p, row, t.half, t.down);
+    return;
+  }
   const int lane = threadIdx.x, kq = lane & 3, nb = lane >> 2;
-  const int64_t e = blockIdx.z;
+  const uint32_t kt = blockIdx.x % (uint32_t)a.kt, rt = blockIdx.x / (uint32_t)a.kt % (uint32_t)t.rb;
+  const int64_t e = blockIdx.x / (uint32_t)a.kt / (uint32_t)t.rb;
   if (a.counts && a.counts[e] <= 0) return;
-  const int64_t nt = (int64_t)blockIdx.y * 8 + (nb >> 1);
+  const int64_t nt = (int64_t)rt * 8 + (nb >> 1);
   u32x4 in[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     in[i] = {0, 0, 0, 0};
     if (nt < a.nt)
-      in[i] = *reinterpret_cast<const u32x4*>(a.data + ((e * a.nt + nt) * a.kt + blockIdx.x) * 256 + (kq * 16 + (nb & 1) * 8 + i) * 4);
+      in[i] = *reinterpret_cast<const u32x4*>(a.data + ((e * a.nt + nt) * a.kt + kt) * 256 + (kq * 16 + (nb & 1) * 8 + i) * 4);
   }
   uint32_t* flat = reinterpret_cast<uint32_t*>(lds);
 #pragma unroll
@@ -190,19 +235,19 @@ template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t tile = (int64_t)blockIdx.x * 8 + i;
+    const int64_t tile = (int64_t)kt * 8 + i;
     if (tile < t.ct) {
       const int pos = i * 64 + lane;
-      reinterpret_cast<u32x4*>(t.out)[((e * t.ct + tile) * t.rb + blockIdx.y) * 64 + lane] = lds[pos ^ ((pos >> 4 & 3) | (pos >> 6 & 1) << 2)];
+      reinterpret_cast<u32x4*>(t.out)[((e * t.ct + tile) * t.rb + rt) * 64 + lane] = lds[pos ^ ((pos >> 4 & 3) | (pos >> 6 & 1) << 2)];
     }
   }
   // scales of the groups that begin in this block of columns
-  const float up = t.half ? a.norm[e] : 1.0f;
+  const float up = a.norm[e];
   for (int j = 0; j < 4; ++j) {
-    const int step = blockIdx.x * 4 + j, grp = w4_group(a, step);
+    const int step = kt * 4 + j, grp = w4_group(a, step);
     if (grp * a.gu != step || grp >= a.gp) continue;
     for (int i = lane; i < 128; i += 64) {
-      const int64_t n = (int64_t)blockIdx.y * 128 + i, tile = n >> 4;
+      const int64_t n = (int64_t)rt * 128 + i, tile = n >> 4;
       float s = 0, z = 0;
       if (tile < a.nt) {
         const int64_t at = ((e * a.nt + tile) * a.gp + grp) * 16 + (n & 15);
@@ -215,13 +260,8 @@ template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args
         }
       }
       const int64_t to = (e * a.gp + grp) * t.rb * 128 + n;
-      static_cast<uint16_t*>(t.ts)[to] = W4F16::from_f32(s * up);
-      if constexpr (KIND == W4_U4) {
-        if (t.half)
-          static_cast<uint16_t*>(t.tz)[to] = W4F16::from_f32(z);
-        else
-          static_cast<float*>(t.tz)[to] = s * z;  // exact: 11 x 11 bits
-      }
+      t.ts[to] = W4F16::from_f32(s * up);  // exact, but for scales more than 2^25 below the expert's largest
+      if constexpr (KIND == W4_U4) t.tz[to] = W4F16::from_f32(z);
     }
   }
 }
@@ -407,8 +447,8 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 size_t turned_bytes(const mq_w4* w) { return up256((size_t)w->experts * w4_ntiles(w->k) * w4_ktiles(w->n) * 1024); }
-size_t turned_params_bytes(const mq_w4* w) {  // of one of the two arrays, float32 at most
-  return up256((size_t)w->experts * groups_padded(w) * w4_ktiles(w->n) * 128 * 4);
+size_t turned_params_bytes(const mq_w4* w) {  // of one of the two arrays
+  return up256((size_t)w->experts * groups_padded(w) * w4_ktiles(w->n) * 128 * 2);
 }
 size_t turn_bytes(const mq_w4* w) { return turned_bytes(w) + 2 * turned_params_bytes(w); }
 size_t part_bytes(const W4Product& p, int64_t rows) {
@@ -453,10 +493,12 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   // (a launch counts its threads in 32 bits)
   if ((int64_t)p.nblocks * p.mblocks * (pl.bm ? 512 : 64 * pl.waves) >= (int64_t)1 << 32) return MQ_ERR_TOO_LARGE;
   p.vec = (uintptr_t)x % 16 == 0 && (ldx % 8 == 0 || rows == 1) && kc % 8 == 0;
-  // workspace: the turned operand (gradient) or the row sums, the splits' partial sums, the padded rows
+  const bool halved = grad && dtype == MQ_BF16;
+  // workspace: the turned operand (gradient) or the row sums, the splits' partial sums, the padded or halved rows and the
+  // factors of the latter
   const size_t sums = sums_bytes(w, pl, p, rows, grad), turned = grad ? turn_bytes(w) : sums;
-  const size_t padded = !p.vec || kc % 128 || (ldx > kMaxStride && rows > 1) ? (size_t)rows * p.rb * 256 : 0;
-  const size_t need = turned + part_bytes(p, rows) + padded;
+  const size_t padded = halved || !p.vec || kc % 128 || (ldx > kMaxStride && rows > 1) ? (size_t)rows * p.rb * 256 : 0;
+  const size_t need = turned + part_bytes(p, rows) + padded + (halved ? (size_t)rows * 4 : 0);
   if (need && (!ws || ws_bytes < need)) return MQ_ERR_WORKSPACE;
   if ((uintptr_t)ws % 16) return MQ_ERR_ALIGN;
   p.x = static_cast<const uint16_t*>(x);
@@ -467,30 +509,44 @@ int product(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t 
   p.part = p.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(ws) + turned) : nullptr;
   p.xs = sums ? static_cast<float*>(ws) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  uint16_t* copy = nullptr;  // the rows that the product reads instead of x
   if (padded) {
     uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + turned + part_bytes(p, rows));
-    hipLaunchKernelGGL(k_w4_pad, dim3((unsigned)((rows + 15) / 16), p.rb), dim3(256), 0, st, p, rows, to);
-    MQ_HIP(hipGetLastError());
-    p.x = to;
-    p.ldx = (int64_t)p.rb * 128;
-    p.kc = p.ldx;
-    p.vec = 1;
+    if (!halved) {
+      hipLaunchKernelGGL(k_w4_pad, dim3((unsigned)((rows + 15) / 16), p.rb), dim3(256), 0, st, p, rows, to);
+      MQ_HIP(hipGetLastError());
+    }
+    copy = to;
   }
   if (grad) {
     char* at = static_cast<char*>(ws);
-    const TurnArgs t = {reinterpret_cast<uint32_t*>(at), at + turned_bytes(w), at + turned_bytes(w) + turned_params_bytes(w),
-                        p.ct, p.rb, dtype == MQ_F16};
-    const dim3 grid(a.kt, p.rb, (unsigned)w->experts);
+    uint16_t* scales = reinterpret_cast<uint16_t*>(at + turned_bytes(w));
+    TurnArgs t = {reinterpret_cast<uint32_t*>(at), scales, scales + turned_params_bytes(w) / 2, p.ct, p.rb, 0, nullptr, nullptr};
+    const int64_t blocks = (int64_t)a.kt * p.rb * w->experts, more = halved ? (rows < 65536 ? rows : 65536) : 0;
+    if ((blocks + more) * 64 >= (int64_t)1 << 32) return MQ_ERR_TOO_LARGE;
+    t.blocks = (uint32_t)blocks;
+    if (halved) {
+      t.half = copy;
+      t.down = reinterpret_cast<float*>(reinterpret_cast<char*>(copy) + padded);
+      p.down = t.down;
+    }
+    const dim3 grid((unsigned)(blocks + more));
     switch (w->kind) {
-      case W4_U4: hipLaunchKernelGGL((k_w4_turn<W4_U4>), grid, dim3(64), 0, st, a, t); break;
-      case W4_S4: hipLaunchKernelGGL((k_w4_turn<W4_S4>), grid, dim3(64), 0, st, a, t); break;
-      case W4_LUT: hipLaunchKernelGGL((k_w4_turn<W4_LUT>), grid, dim3(64), 0, st, a, t); break;
-      default: hipLaunchKernelGGL((k_w4_turn<W4_FP4>), grid, dim3(64), 0, st, a, t); break;
+      case W4_U4: hipLaunchKernelGGL((k_w4_turn<W4_U4>), grid, dim3(64), 0, st, a, t, p); break;
+      case W4_S4: hipLaunchKernelGGL((k_w4_turn<W4_S4>), grid, dim3(64), 0, st, a, t, p); break;
+      case W4_LUT: hipLaunchKernelGGL((k_w4_turn<W4_LUT>), grid, dim3(64), 0, st, a, t, p); break;
+      default: hipLaunchKernelGGL((k_w4_turn<W4_FP4>), grid, dim3(64), 0, st, a, t, p); break;
     }
     MQ_HIP(hipGetLastError());
     p.b = t.out;
     p.ts = t.ts;
     p.tz = t.tz;
+  }
+  if (copy) {
+    p.x = copy;
+    p.ldx = (int64_t)p.rb * 128;
+    p.kc = p.ldx;
+    p.vec = 1;
   }
   const bool h = dtype == MQ_F16;
   hipError_t e;
@@ -590,14 +646,16 @@ extern "C" int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream) {
   }
   return MQ_OK;
 }
-extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int64_t rows, int32_t aligned, int32_t counted, int32_t grad) {
+extern "C" size_t mq_linear4_workspace_bytes(const mq_w4* w, int32_t dtype, int64_t rows, int32_t aligned, int32_t counted,
+                                             int32_t grad) {
   if (check_w4(w) != MQ_OK || rows < 1 || rows > kMaxRows) return 0;
   size_t need = grad & 2 ? bias_bytes(w, rows) : 0;
   if (grad == 2) return need;
   W4Product p = {};
   const W4Plan pl = plan_of(w, rows, grad != 0, counted != 0, &p);
   need += (grad ? turn_bytes(w) : sums_bytes(w, pl, p, rows, false)) + part_bytes(p, rows);
-  return need + (!aligned || p.kc % 128 ? (size_t)rows * p.rb * 256 : 0);
+  const bool halved = grad && dtype == MQ_BF16;
+  return need + (halved || !aligned || p.kc % 128 ? (size_t)rows * p.rb * 256 : 0) + (halved ? (size_t)rows * 4 : 0);
 }
 extern "C" int mq_linear4(const mq_w4* w, const void* x, int32_t dtype, int64_t rows, int64_t ldx, const void* bias,
                           const int32_t* counts, void* y, void* workspace, size_t workspace_bytes, void* hip_stream) {

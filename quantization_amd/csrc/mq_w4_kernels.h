@@ -11,8 +11,9 @@ struct W4Product {
   uint16_t* y;           // [rows][nc]
   float* part;           // [splits][rows][16 * ct] partial sums, NULL when splits == 1
   float* xs;             // sums of x per window and row (k_w4_rowsum), for zero points in k_w4_gemm
-  const void* ts;        // gradient: scales along the contraction, k_w4_turn's [E][GP][128 rb]
-  const void* tz;        // ... and zero points (float16) or scale * zero (bfloat16)
+  const uint16_t* ts;    // gradient: scales along the contraction times norm, k_w4_turn's [E][GP][128 rb]
+  const uint16_t* tz;    // ... and zero points
+  const float* down;     // gradient of bfloat16: what k_w4_half's rows have to be multiplied by
   int64_t ldx, kc, nc;   // contraction length, output columns
   int32_t ct, rb;        // 16-column tiles of the output, 128-blocks of the contraction
   int32_t vec;           // rows of x are 16-byte aligned and kc % 8 == 0
@@ -209,43 +210,20 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_w4_rows(const W4A
 }
 
 // ---- the gradient's scaled weights ---------------------------------------------------------------------
-// Eight weights of one column, scale * (q - zero) rounded once to T.  float16: the integer difference is exact, the
-// product rounds (scales are held times the expert's norm, a power of two); bfloat16: one float32 fma, then the rounding.
-template <class T, int KIND> struct W4Scales;
-template <int KIND> struct W4Scales<W4F16, KIND> {
+// Eight weights of one column in float16, scale * (q - zero) times the expert's norm (a power of two): the difference of
+// integers is exact, the product rounds once (2^-11 of the weight at most).
+template <int KIND> struct W4Scales {
   u32x4 s, z;
   __device__ __forceinline__ void load(const W4Product& p, int64_t at) {
-    s = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.ts) + at);
-    if constexpr (KIND == W4_U4) z = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.tz) + at);
+    s = *reinterpret_cast<const u32x4*>(p.ts + at);
+    if constexpr (KIND == W4_U4) z = *reinterpret_cast<const u32x4*>(p.tz + at);
   }
   __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
-    u32x4 v = w4_decode<W4F16, KIND>(d, lut);
+    const u32x4 v = w4_decode<W4F16, KIND>(d, lut);
     // (whole vectors: the compiler takes a bit cast of one element of a vector for one of its first element)
     w4_h8 q = __builtin_bit_cast(w4_h8, v);
     if constexpr (KIND == W4_U4) q = q - __builtin_bit_cast(w4_h8, z);
     return __builtin_bit_cast(u32x4, q * __builtin_bit_cast(w4_h8, s));
-  }
-};
-template <int KIND> struct W4Scales<W4BF16, KIND> {
-  u32x4 s;     // float16 as they are: v_fma_mix_f32 takes them so, and half the bytes come through the cache
-  f32x4 z[2];  // scale * zero
-  __device__ __forceinline__ void load(const W4Product& p, int64_t at) {
-    s = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.ts) + at);
-    if constexpr (KIND == W4_U4) {
-      const f32x4* zero = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.tz) + at);
-      z[0] = zero[0], z[1] = zero[1];
-    }
-  }
-  __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
-    float f[8];
-    w4_decode_f32<KIND>(d, lut, f);
-    const w4_h8 h = __builtin_bit_cast(w4_h8, s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __builtin_fmaf(f[i], (float)h[i], KIND == W4_U4 ? -z[i / 4][i % 4] : 0.0f);
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = W4BF16::pack(f[2 * i], f[2 * i + 1]);
-    return v;
   }
 };
 
@@ -262,7 +240,9 @@ template <int KIND> struct W4Scales<W4BF16, KIND> {
 // Rows are 16-byte aligned and a multiple of 128 long here: others are copied first (k_w4_pad).
 // GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.
 // GRAD = true (dx = dy W, operand b transposed): scales change along the contraction, so they are multiplied into the
-// weights, which are rounded once to T -- half a step of T per weight, as a weight stored in T has.
+// weights, which are rounded once to float16 (W4Scales).  It runs in float16 for both types: rows of bfloat16 are brought
+// into its range by a power of two each (k_w4_half), where they lose nothing, while weights rounded to bfloat16 would add
+// as much error as the rounding of the result (2.4e-3 of the norm against 1.7e-3) and take more instructions to make.
 template <int NT, int W> struct W4Ahead {  // what a wave holds of a block that is on its way
   u32x4 b[NT][2];
   uint32_t s[NT][W];
@@ -275,7 +255,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_buffer(const void* base, ui
 #endif
 typedef __attribute__((address_space(3))) void w4_lds_t;
 
-template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int WK, int FS>
+template <class T, class TO, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int WK, int FS>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a, const W4Product p) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass has no buffer descriptors; it needs the kernel's name only)
   constexpr int BM = 32 * MT * WM, NW = WM * WN, CH = BM / 4 / NW;  // 1 KiB pieces (4 rows) per wave
@@ -427,7 +407,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
         constexpr int SETS = FS == 1 ? NT : 1;  // groups under a wave's 32 NT columns
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
-          W4Scales<T, KIND> sc[SETS];
+          W4Scales<KIND> sc[SETS];
 #pragma unroll
           for (int g = 0; g < SETS; ++g) sc[g].load(p, st0[g] + kb * 128 + st * 16);
           u32x4 xv[MT];
@@ -444,13 +424,19 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       __syncthreads();
     }
     if constexpr (GRAD) {
-      const float down = T::kHalf ? 1.0f / a.norm[expert] : 1.0f;  // (float16 weights are held times norm, a power of two)
+      const float down = 1.0f / a.norm[expert];  // a power of two, as are the rows' factors
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int q = 0; q < 4; ++q) {
+          const int r = (wm * MT + m) * 32 + q * 8 + half * 4;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sum[m][n][i] = acc[m][n][i] * down;
+          for (int i = 0; i < 4; ++i) {
+            const float row = TO::kHalf ? 1.0f : p.down[row0 + (r + i < rows ? r + i : rows - 1)];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sum[m][n][4 * q + i] = acc[m][n][4 * q + i] * down * row;
+          }
+        }
     }
   }
   if constexpr (WK > 1) {  // the halves' sums, through the buffers that nobody reads any more
@@ -479,8 +465,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
     const int64_t col = (tile0 + n) * 32 + (l32 & ~1);
     float b0 = 0, b1 = 0;
     if (p.bias && expert >= 0 && blockIdx.y == 0) {
-      if (col < p.nc) b0 = T::to_f32(p.bias[expert * p.nc + col]);
-      if (col + 1 < p.nc) b1 = T::to_f32(p.bias[expert * p.nc + col + 1]);
+      if (col < p.nc) b0 = TO::to_f32(p.bias[expert * p.nc + col]);
+      if (col + 1 < p.nc) b1 = TO::to_f32(p.bias[expert * p.nc + col + 1]);
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -499,10 +485,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
           } else {
             uint16_t* to = p.y + (row0 + r) * p.nc + col;
             if (p.nc % 2 == 0) {
-              *reinterpret_cast<uint32_t*>(to) = T::pack(v0, v1);
+              *reinterpret_cast<uint32_t*>(to) = TO::pack(v0, v1);
             } else {
-              to[0] = T::from_f32(v0);
-              if (col + 1 < p.nc) to[1] = T::from_f32(v1);
+              to[0] = TO::from_f32(v0);
+              if (col + 1 < p.nc) to[1] = TO::from_f32(v1);
             }
           }
         }
@@ -557,20 +543,20 @@ static void w4_rows_go(const W4Args& a, const W4Product& p, const W4Plan& pl, hi
   else
     hipLaunchKernelGGL((k_w4_rows<T, KIND, MT, NT, 1>), grid, block, lds, st, a, p);
 }
-template <class T, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int WK>
+template <class T, class TO, int KIND, bool GRAD, int MT, int NT, int WM, int WN, int WK>
 static void w4_gemm_go(const W4Args& a, const W4Product& p, const W4Plan& pl, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)p.nblocks * p.mblocks), p.splits), block(64 * WM * WN * WK);
   const dim3 sums((unsigned)((a.rows + 15) / 16), p.rb);
   constexpr bool xs = KIND == W4_U4 && !GRAD;
   if (GRAD ? pl.fs >= 2 : pl.fs == 4) {
     if (xs) hipLaunchKernelGGL((k_w4_rowsum<T, 4>), sums, dim3(256), 0, st, p, a.rows, p.xs);
-    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, WK, 4>), grid, block, 0, st, a, p);
+    hipLaunchKernelGGL((k_w4_gemm<T, TO, KIND, GRAD, MT, NT, WM, WN, WK, 4>), grid, block, 0, st, a, p);
   } else if (!GRAD && pl.fs == 2) {
     if (xs) hipLaunchKernelGGL((k_w4_rowsum<T, 2>), sums, dim3(256), 0, st, p, a.rows, p.xs);
-    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, WK, GRAD ? 4 : 2>), grid, block, 0, st, a, p);
+    hipLaunchKernelGGL((k_w4_gemm<T, TO, KIND, GRAD, MT, NT, WM, WN, WK, GRAD ? 4 : 2>), grid, block, 0, st, a, p);
   } else {
     if (xs) hipLaunchKernelGGL((k_w4_rowsum<T, 1>), sums, dim3(256), 0, st, p, a.rows, p.xs);
-    hipLaunchKernelGGL((k_w4_gemm<T, KIND, GRAD, MT, NT, WM, WN, WK, 1>), grid, block, 0, st, a, p);
+    hipLaunchKernelGGL((k_w4_gemm<T, TO, KIND, GRAD, MT, NT, WM, WN, WK, 1>), grid, block, 0, st, a, p);
   }
 }
 
@@ -584,11 +570,11 @@ hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool
     else if (pl.nt == 2) w4_rows_go<T, KIND, 2, 2>(a, p, pl, st);
     else w4_rows_go<T, KIND, 2, 4>(a, p, pl, st);
   } else if (grad) {
-    if (pl.bm == 64) w4_gemm_go<T, KIND, true, 1, 2, 2, 2, 2>(a, p, pl, st);
-    else w4_gemm_go<T, KIND, true, 4, 2, 1, 4, 1>(a, p, pl, st);
+    if (pl.bm == 64) w4_gemm_go<W4F16, T, KIND, true, 1, 2, 2, 2, 2>(a, p, pl, st);
+    else w4_gemm_go<W4F16, T, KIND, true, 4, 2, 1, 4, 1>(a, p, pl, st);
   } else {
-    if (pl.bm == 64) w4_gemm_go<T, KIND, false, 1, 2, 2, 2, 2>(a, p, pl, st);
-    else w4_gemm_go<T, KIND, false, 2, 2, 2, 2, 1>(a, p, pl, st);
+    if (pl.bm == 64) w4_gemm_go<T, T, KIND, false, 1, 2, 2, 2, 2>(a, p, pl, st);
+    else w4_gemm_go<T, T, KIND, false, 2, 2, 2, 2, 1>(a, p, pl, st);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.part) return e;

@@ -44,7 +44,7 @@ def _bind():
         L.mq_w4_params_bytes.restype, L.mq_w4_params_bytes.argtypes = sz, [pw]
         L.mq_w4_pack.restype, L.mq_w4_pack.argtypes = ctypes.c_int, [pw, vp, vp, vp, vp]
         L.mq_w4_unpack.restype, L.mq_w4_unpack.argtypes = ctypes.c_int, [pw, vp, vp]
-        L.mq_linear4_workspace_bytes.restype, L.mq_linear4_workspace_bytes.argtypes = sz, [pw, i64, i32, i32, i32]
+        L.mq_linear4_workspace_bytes.restype, L.mq_linear4_workspace_bytes.argtypes = sz, [pw, i32, i64, i32, i32, i32]
         L.mq_linear4.restype, L.mq_linear4.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, vp, sz, vp]
         L.mq_linear4_grad.restype, L.mq_linear4_grad.argtypes = ctypes.c_int, [pw, vp, i32, i64, i64, vp, vp, vp, vp, sz, vp]
         _bound = L
@@ -119,7 +119,7 @@ class PackedWeight:
                 raise ValueError(f"not the tensors of a packed weight: {t.dtype} {tuple(t.shape)} on {t.device}")
         self._c = s
         self._ref = ctypes.byref(s)
-        self._need = {}   # workspace bytes by (rows, aligned, counted, grad)
+        self._need = {}   # workspace bytes by (dtype, rows, aligned, counted, grad)
         self._device = self.data.device
 
     def __getstate__(self):
@@ -276,7 +276,7 @@ def _workspace(weight, t, ld, counts, grad):
     """-> (tensor | None, bytes).  Of this call alone: a captured graph keeps it in its own pool, and calls on other
     streams have their own."""
     rows = t.shape[0]
-    key = (rows, t.data_ptr() % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 23 or rows == 1), counts is not None, grad)
+    key = (_XDTYPES[t.dtype], rows, t.data_ptr() % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 23 or rows == 1), counts is not None, grad)
     need = weight._need.get(key)
     if need is None:
         if len(weight._need) >= 4096:

@@ -4,7 +4,7 @@ Bounds, from the arithmetic: the codes' values enter the products exactly (forwa
 depth = K / 32 + 2 G + 40 float32 roundings on its way into the sum (32 terms are added inside a matrix instruction, one
 sum per 32, one scaled addition per group -- two with a zero point -- and the waves' or splits' sums), each at most 2^-23
 of the terms' absolute sum; the result is rounded once: eps / 2 of itself.  In the backward product every weight is first
-rounded once: eps / 2 of the terms' absolute sum.  Results below the type's normal numbers are off by half their step."""
+rounded once, to float16 (11 significant bits, half a step: 2^-11 of it at most), so 2^-11 of the terms' absolute sum.  Results below the type's normal numbers are off by half their step."""
 import copy
 
 import pytest
@@ -55,7 +55,7 @@ def depth(k, p):
 
 def near(got, want, mass, k, p, rounded=False, what=""):
     eps = torch.finfo(got.dtype).eps / 2
-    tol = eps * want.abs() + (depth(k, p) + (eps if rounded else 0)) * (1 + eps) * mass
+    tol = eps * want.abs() + (depth(k, p) + (2.0 ** -11 if rounded else 0)) * (1 + eps) * mass
     tol = tol + torch.finfo(got.dtype).smallest_normal * eps
     off = (got.double() - want).abs()
     bad = off > tol
@@ -306,6 +306,26 @@ def test_a_row_that_is_not_finite_stays_its_own(pk):
             assert y[2].isnan().all() and not y[4].isfinite().any()
             keep = [i for i in range(m) if i not in (2, 4)]
             near(y[keep], product(x[keep], w), product(x[keep].abs(), mass), 256, p, what=(fmt, m))
+
+
+def test_gradients_of_every_size(pk):
+    """Rows of dy of very different size, up to both ends of bfloat16, in one call: each keeps its bits."""
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    n, k = 200, 128
+    p, w, _, _ = weight(gen, (n, k), "int4", 4, 32)
+    for m in (30, 200):
+        size = torch.logspace(-37, 36, m, device="cuda", dtype=torch.float64)[:, None]
+        dy = (torch.randn(m, n, generator=gen, device="cuda").double() * size).bfloat16()
+        dy[3], dy[5, 1:] = 0, 0
+        x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        dx, = torch.autograd.grad(pk.packed_linear(x, p), x, dy)
+        near(dx, product(dy, w.t()), product(dy.abs(), w.t().abs()), n, p, rounded=True, what=m)
+        assert not dx[3].any()
+        dy[7, 9], dy[8, 9] = float("inf"), float("nan")
+        dx, = torch.autograd.grad(pk.packed_linear(x, p), x, dy)
+        assert not dx[7:9].isfinite().any()
+        keep = [i for i in range(m) if i not in (7, 8)]
+        near(dx[keep], product(dy[keep], w.t()), product(dy[keep].abs(), w.t().abs()), n, p, rounded=True, what=m)
 
 
 def test_streams_and_graphs(pk):

@@ -62,7 +62,7 @@ def test_library_refuses_before_any_launch():
     bad.values[0], bad.values[1] = 1.0, 1.0
     assert call(bad) == _lib.ERR_UNSUPPORTED                    # entry 0 is what padding decodes to
     assert call(_c(n=1 << 22, k=1 << 20, group=0), rows=1 << 27, ld=1 << 20) in (_lib.ERR_TOO_LARGE, _lib.ERR_WORKSPACE)
-    need = L.mq_linear4_workspace_bytes(ref(_c()), 4, 1, 0, 1)     # the gradient's turned operand
+    need = L.mq_linear4_workspace_bytes(ref(_c()), _lib.F16, 4, 1, 0, 1)     # the gradient's turned operand
     assert need >= 16 * 1024
     back = lambda dx, db, ws, size, c=_c(), dt=_lib.F16: L.mq_linear4_grad(ref(c), 4096, dt, 4, 64, None, dx, db, ws, size, None)
     assert back(4096, None, None, 0) == _lib.ERR_WORKSPACE
@@ -71,8 +71,8 @@ def test_library_refuses_before_any_launch():
     assert back(None, 4097, 4096, big) == _lib.ERR_ALIGN
     assert back(None, 4096, 4096, big, dt=_lib.F32) == _lib.ERR_UNSUPPORTED
     assert back(None, 4096, 4096, big, c=_c(experts=3)) == _lib.ERR_ARG
-    assert L.mq_linear4_workspace_bytes(ref(_c()), 4, 1, 0, 2) == 0
-    assert L.mq_linear4_workspace_bytes(ref(_c()), 4096, 1, 0, 2) > 0      # runs of rows, added by a second launch
+    assert L.mq_linear4_workspace_bytes(ref(_c()), _lib.F16, 4, 1, 0, 2) == 0
+    assert L.mq_linear4_workspace_bytes(ref(_c()), _lib.F16, 4096, 1, 0, 2) > 0      # runs of rows, added by a second launch
     assert L.mq_w4_pack(ref(_c()), None, 4096, None, None) == _lib.ERR_ARG
     assert L.mq_w4_pack(ref(_c()), 4096, 4096, 4096, None) == _lib.ERR_ARG         # a zero point with symmetric codes
     assert L.mq_w4_unpack(ref(_c()), None, None) == _lib.ERR_ARG
