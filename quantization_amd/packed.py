@@ -258,9 +258,12 @@ def pack_weight(w, wq_bits: int = 4, datatype: str = "int4", group_size=None) ->
 
 def _rows_of(t):
     """A 2-D tensor as (tensor, elements from row to row) with neighbouring columns side by side."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and 0 < t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    if t.is_contiguous() or rows == 1 and (cols == 1 or t.stride(1) == 1):
+        return t, cols
+    if cols > 1 and t.stride(1) != 1 or 0 < t.stride(0) < cols:
+        return t.contiguous(), cols
+    return t, t.stride(0)
 
 
 def _on_device(call, t, *args):
@@ -272,17 +275,19 @@ def _on_device(call, t, *args):
         return call(t, *args, index)
 
 
-def _workspace(weight, t, ld, counts, grad):
-    """-> (tensor | None, bytes).  Of this call alone: a captured graph keeps it in its own pool, and calls on other
-    streams have their own."""
-    rows = t.shape[0]
-    key = (_XDTYPES[t.dtype], rows, t.data_ptr() % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 23 or rows == 1), counts is not None, grad)
+def _workspace(weight, t, at, rows, ld, counts, grad):
+    """-> (tensor | None, its address, bytes).  Of this call alone: a captured graph keeps it in its own pool, and calls on
+    other streams have their own."""
+    key = (_XDTYPES[t.dtype], rows, at % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 23 or rows == 1), counts is not None, grad)
     need = weight._need.get(key)
     if need is None:
         if len(weight._need) >= 4096:
             weight._need.clear()
         need = weight._need[key] = _bound.mq_linear4_workspace_bytes(weight._ref, *key)
-    return (torch.empty(need, dtype=torch.uint8, device=t.device) if need else None), need
+    if not need:
+        return None, None, 0
+    ws = torch.empty(need, dtype=torch.uint8, device=t.device)
+    return ws, ws.data_ptr(), need
 
 
 def _forward(x, weight, bias, counts, index):
@@ -291,10 +296,11 @@ def _forward(x, weight, bias, counts, index):
     y = x.new_empty((rows, weight.n))
     if rows:
         x, ld = _rows_of(x)
-        ws, need = _workspace(weight, x, ld, counts, 0)
-        rc = L.mq_linear4(weight._ref, x.data_ptr(), _XDTYPES[x.dtype], rows, ld, None if bias is None else bias.data_ptr(),
-                          None if counts is None else counts.data_ptr(), y.data_ptr(), None if ws is None else ws.data_ptr(),
-                          need, torch._C._cuda_getCurrentRawStream(index))
+        at = x.data_ptr()
+        ws, wp, need = _workspace(weight, x, at, rows, ld, counts, 0)
+        rc = L.mq_linear4(weight._ref, at, _XDTYPES[x.dtype], rows, ld, None if bias is None else bias.data_ptr(),
+                          None if counts is None else counts.data_ptr(), y.data_ptr(), wp, need,
+                          torch._C._cuda_getCurrentRawStream(index))
         if rc:
             _lib.check(rc)
     return y
@@ -308,10 +314,11 @@ def _backward(dy, weight, counts, want_x, want_bias, index):
     if not rows:
         return dx, None if db is None else db.zero_()
     dy, ld = _rows_of(dy)
-    ws, need = _workspace(weight, dy, ld, counts, want_x + 2 * want_bias)
-    rc = L.mq_linear4_grad(weight._ref, dy.data_ptr(), _XDTYPES[dy.dtype], rows, ld, None if counts is None else counts.data_ptr(),
-                           None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(),
-                           None if ws is None else ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index))
+    at = dy.data_ptr()
+    ws, wp, need = _workspace(weight, dy, at, rows, ld, counts, want_x + 2 * want_bias)
+    rc = L.mq_linear4_grad(weight._ref, at, _XDTYPES[dy.dtype], rows, ld, None if counts is None else counts.data_ptr(),
+                           None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), wp, need,
+                           torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc)
     return dx, db
