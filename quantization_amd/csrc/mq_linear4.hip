@@ -418,25 +418,28 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
     return pl;
   }
   // Tile height and cuts of the contraction (pieces of at least 4 blocks of 128, joined by a second launch): the cheapest
-  // by what was measured on 4096 x 4096, microseconds per block of 128 for a compute unit with one tile and with two.
-  // 64 x 128: 0.7 and 1.55 (gradient 1.5 and 2.9), 128 x 128: 1.3 and 2.3, the gradient's 128 x 256: 3.4 and 5.0 (it
-  // decodes half as often per product, which is what bounds it: 4096 rows 162 against 235 with 128 x 128).  A tile begins
-  // and ends in 1.5; a join takes 3 and moves its sums at about 4 MB per microsecond.
-  static const double kTime[2][2][2] = {{{0.7, 1.55}, {1.3, 2.3}}, {{1.5, 2.9}, {3.4, 5.0}}};
+  // by what was measured on 4096 x 4096, microseconds per block of 128 for a compute unit with one tile (two sets of waves
+  // in it), with two, and for an odd one behind pairs.  64 x 128: 0.7, 1.55, 0.7 (gradient 1.5, 2.9, 1.5), 128 x 128:
+  // 1.2, 2.3, 1.3, the gradient's 128 x 256: 2.6, 5.0, 3.4 (it decodes half as often per product: 4096 rows 162 against 235
+  // with 128 x 128; one tile with one set of waves takes 3.4, pairs with two sets 5.6).  A tile begins and ends in 1.5; a
+  // join takes 3 and moves its sums at about 4 MB per microsecond.
+  static const double kTime[2][2][3] = {{{0.7, 1.55, 0.7}, {1.2, 2.3, 1.3}}, {{1.5, 2.9, 1.5}, {2.6, 5.0, 3.4}}};
   double best = 0;
   for (int tall = 0; tall < 2; ++tall) {
     const int bm = tall ? 128 : 64, bn = tall && grad ? 256 : 128;
     const int64_t nblocks = (p->ct * 16 + bn - 1) / bn;
     // (the last tile of an expert is half full on average)
     const int64_t tiles = (counted ? rows / bm + (busy + 1) / 2 : (rows + bm - 1) / bm) * nblocks;
+    const double* time = kTime[grad][tall];
     for (int s = 1; s <= 8 && (s == 1 || p->rb >= 4 * s); s *= 2) {
       const int64_t each = (tiles * s + 255) / 256;  // tiles of a compute unit
-      const double t = (each / 2 * kTime[grad][tall][1] + each % 2 * kTime[grad][tall][0]) * p->rb / s + 1.5 * each +
+      const double t = (each == 1 ? time[0] : each / 2 * time[1] + each % 2 * time[2]) * p->rb / s + 1.5 * each +
                        (s > 1 ? 3 + 8e-6 * s * rows * p->ct * 16 / 4 : 0);
       if (pl.bm && t >= best) continue;
       best = t;
       pl.bm = bm;
       pl.bn = bn;
+      pl.wk = each == 1 ? 2 : 1;
       p->splits = s;
       p->nblocks = (int32_t)nblocks;
     }

@@ -235,8 +235,8 @@ template <int KIND> struct W4Scales {
 // fetched in whole lines and neither the writes nor the operand reads meet in a bank.  The packed weight goes from memory
 // straight into the registers of the wave that decodes it: lane l takes row l % 32 of the 32-row tile, the halves of its
 // wave the eight columns 8 (l / 32) of every sixteen -- two of the layout's four dwords-quadruples.
-// WK = 2: two sets of waves with buffers of their own take the blocks of the contraction in turn, for small tiles, where
-// one wave per SIMD would wait for its own decoding.
+// WK = 2: two sets of waves with buffers of their own take the blocks of the contraction in turn, for small tiles and where
+// a compute unit has only one: one wave per SIMD would wait for its own decoding.
 // Rows are 16-byte aligned and a multiple of 128 long here: others are copied first (k_w4_pad).
 // GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.
 // GRAD = true (dx = dy W, operand b transposed): scales change along the contraction, so they are multiplied into the
@@ -528,7 +528,7 @@ template <class T> __global__ __launch_bounds__(256) void k_w4_join(const W4Prod
 // ---- launchers: one set per (type, kind) -------------------------------------------------------------
 struct W4Plan {
   int mt, nt, waves;  // k_w4_rows
-  int bm, bn;         // k_w4_gemm (bm = 0: k_w4_rows)
+  int bm, bn, wk;     // k_w4_gemm (bm = 0: k_w4_rows)
   int fs;
 };
 
@@ -571,9 +571,11 @@ hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool
     else w4_rows_go<T, KIND, 2, 4>(a, p, pl, st);
   } else if (grad) {
     if (pl.bm == 64) w4_gemm_go<W4F16, T, KIND, true, 1, 2, 2, 2, 2>(a, p, pl, st);
+    else if (pl.wk == 2) w4_gemm_go<W4F16, T, KIND, true, 4, 2, 1, 4, 2>(a, p, pl, st);
     else w4_gemm_go<W4F16, T, KIND, true, 4, 2, 1, 4, 1>(a, p, pl, st);
   } else {
     if (pl.bm == 64) w4_gemm_go<T, T, KIND, false, 1, 2, 2, 2, 2>(a, p, pl, st);
+    else if (pl.wk == 2) w4_gemm_go<T, T, KIND, false, 2, 2, 2, 2, 2>(a, p, pl, st);
     else w4_gemm_go<T, T, KIND, false, 2, 2, 2, 2, 1>(a, p, pl, st);
   }
   hipError_t e = hipGetLastError();
