@@ -459,7 +459,7 @@ size_t part_bytes(const W4Product& p, int64_t rows) {
 }
 // the row sums for the zero points (k_w4_rowsum)
 size_t sums_bytes(const mq_w4* w, const W4Plan& pl, const W4Product& p, int64_t rows, bool grad) {
-  return pl.bm && !grad && w->kind == W4_U4 ? up256(((size_t)p.rb * (4 / pl.fs) * rows + pl.bm) * 4) : 0;  // (a tile reads past the last row)
+  return pl.bm && !grad && w->kind == W4_U4 ? up256((size_t)p.rb * (4 / pl.fs) * rows * 4) : 0;
 }
 
 int32_t bias_splits(int64_t rows, int64_t experts) {

@@ -238,7 +238,10 @@ template <int KIND> struct W4Scales {
 // WK = 2: two sets of waves with buffers of their own take the blocks of the contraction in turn, for small tiles and where
 // a compute unit has only one: one wave per SIMD would wait for its own decoding.
 // Rows are 16-byte aligned and a multiple of 128 long here: others are copied first (k_w4_pad).
-// GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.
+// GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.  Zero
+// points: minus (scale * zero)[column] * (sum of x)[row] per window of FS steps, a float32 product on the matrix cores
+// with a contraction over the windows (v_mfma_f32_32x32x2_f32): done by the vector units it took as many instructions
+// again as the scaling.
 // GRAD = true (dx = dy W, operand b transposed): scales change along the contraction, so they are multiplied into the
 // weights, which are rounded once to float16 (W4Scales).  It runs in float16 for both types: rows of bfloat16 are brought
 // into its range by a power of two each (k_w4_half), where they lose nothing, while weights rounded to bfloat16 would add
@@ -260,14 +263,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass has no buffer descriptors; it needs the kernel's name only)
   constexpr int BM = 32 * MT * WM, NW = WM * WN, CH = BM / 4 / NW;  // 1 KiB pieces (4 rows) per wave
   constexpr int W = 4 / FS;                                         // windows of a block with a scale each
-  constexpr bool XS = KIND == W4_U4 && !GRAD;
+  constexpr bool XS = KIND == W4_U4 && !GRAD;                       // zero points, taken away through the rows' sums
+  constexpr int PAIRS = W == 4 ? 2 : 1;
   static_assert(BM / 4 % NW == 0 && BM % 64 == 0, "the rows of a block are dealt evenly");
   __shared__ u32x4 lds_all[WK][2][BM * 16];
-  __shared__ f32x4 lds_xs_all[WK][XS ? 2 : 1][XS ? W * BM / 4 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int w = wave % NW, wk = wave / NW, wm = w % WM, wn = w / WM;
   auto& lds = lds_all[wk];
-  auto& lds_xs = lds_xs_all[wk];
   // Workgroups go to the eight chiplets in turn: row tile 8 i + c belongs to chiplet c, whose L2 then holds its rows for all
   // columns; the row tiles behind the last eight are dealt out by columns.
   const uint32_t whole = (uint32_t)p.mblocks / 8 * (uint32_t)p.nblocks * 8, id = blockIdx.x;
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
   int expert, rows;
   int64_t row0;
   if (!w4_find_tile(a, BM, mb, expert, row0, rows)) return;
-  f32x16 acc[MT][NT];     // GRAD: the matrix instructions' own sums
+  f32x16 acc[MT][NT];     // GRAD, zero points: the matrix instructions' own sums
   float sum[MT][NT][16];  // forward: the scaled sums (single registers: they are never a matrix operand)
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -322,26 +324,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
 #pragma unroll
       for (int c = 0; c < CH; ++c)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xsrc, (w4_lds_t*)&lds[buf][(w * CH + c) * 64], 16, xo[c], kb * 256, 0, 0);
-      if constexpr (XS) {  // 64 row sums to a wave's load; a tile may read past the last row
-#pragma unroll
-        for (int c = 0; c < W * BM / 64; ++c)
-          if (c % NW == w)
-            __builtin_amdgcn_global_load_lds((w4_global_t*)(p.xs + ((int64_t)kb * W + c / (BM / 64)) * a.rows + row0 + c % (BM / 64) * 64 + lane),
-                                             (w4_lds_t*)&lds_xs[buf][c * 16], 4, 0, 0);
-      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) to.b[n][h] = __builtin_amdgcn_raw_buffer_load_b128(bsrc, bo[n] + h * 512, kb * 1024, 0);
         if constexpr (!GRAD) {
 #pragma unroll
-          for (int v = 0; v < W; ++v) {
-            const int64_t at = pt[n] + w4_group(a, kb * 4 + v * FS) * 16;
-            if constexpr (KIND == W4_U4)
-              to.s[n][v] = static_cast<const uint32_t*>(a.params)[at];
-            else
-              to.s[n][v] = static_cast<const uint16_t*>(a.params)[at];
-          }
+          for (int v = 0; v < W; ++v)
+            to.s[n][v] = static_cast<const uint16_t*>(a.params)[(pt[n] + w4_group(a, kb * 4 + v * FS) * 16) * (KIND == W4_U4 ? 2 : 1)];
         }
       }
     };
@@ -362,6 +352,29 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       if (WK > 1 && kb >= kb1) {
         // the other waves' last block: nothing for this half
       } else if constexpr (!GRAD) {
+        // What the zero points take away of two windows at a time -- of this block, or (one window to a block) of every
+        // second block and the one before it: lanes' halves hold a window each.
+        float zx[PAIRS][MT], zz[PAIRS][NT];
+        const bool pair_now = W > 1 || (it & 1) || kb + WK >= kb1;
+        if constexpr (XS) {
+          if (pair_now) {
+#pragma unroll
+            for (int v = 0; v < PAIRS; ++v) {
+              const bool there = W > 1 || (it & 1) || !half;
+              const int win = W > 1 ? kb * W + 2 * v + half : (it & 1) && !half ? kb - WK : kb;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const int r = (wm * MT + m) * 32 + l32;
+                zx[v][m] = p.xs[(int64_t)win * a.rows + row0 + (r < rows ? r : rows - 1)];
+              }
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                const uint32_t q = static_cast<const uint32_t*>(a.params)[pt[n] + w4_group(a, win * FS) * 16];
+                zz[v][n] = there ? -(float)h_from_bits(q) * (float)h_from_bits(q >> 16) : 0.0f;  // exact: 11 x 11 bits
+              }
+            }
+          }
+        }
         f32x16 tmp[MT][NT];
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
@@ -376,31 +389,35 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
           }
           if ((st + 1) % (2 * FS) == 0) {
             const int v = st / (2 * FS);
-            float s[NT], sz[NT];
+            float s[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               s[n] = (float)h_from_bits(cur.s[n][v]);
               asm("" : "+v"(s[n]));  // a float32 register: v_fmac_f32 issues faster than the mixed fma the compiler would choose
-              if constexpr (KIND == W4_U4) sz[n] = -(s[n] * (float)h_from_bits(cur.s[n][v] >> 16));  // exact: 11 x 11 bits
             }
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {  // registers 4 q .. 4 q + 3: rows 8 q + 4 half + (0 .. 3) of the tile
-                f32x4 x = {0, 0, 0, 0};
-                if constexpr (XS) x = lds_xs[buf][v * (BM / 4) + (wm * MT + m) * 8 + q * 2 + half];
+              for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                  for (int n = 0; n < NT; ++n) {
-                    sum[m][n][4 * q + i] = __builtin_fmaf(s[n], tmp[m][n][4 * q + i], sum[m][n][4 * q + i]);
-                    if constexpr (KIND == W4_U4) sum[m][n][4 * q + i] = __builtin_fmaf(sz[n], x[i], sum[m][n][4 * q + i]);
-                  }
+                for (int i = 0; i < 16; ++i) {
+                  if constexpr (XS)
+                    acc[m][n][i] = __builtin_fmaf(s[n], tmp[m][n][i], acc[m][n][i]);
+                  else
+                    sum[m][n][i] = __builtin_fmaf(s[n], tmp[m][n][i], sum[m][n][i]);
                 }
-              }
-            }
             // one window's unscaled sums at a time: without this the scheduler keeps several in registers and spills
             if (FS < 4) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if constexpr (XS) {
+          if (pair_now) {
+#pragma unroll
+            for (int v = 0; v < PAIRS; ++v)
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(zx[v][m], zz[v][n], acc[m][n], 0, 0, 0);
           }
         }
       } else {
@@ -422,6 +439,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
         }
       }
       __syncthreads();
+    }
+    if constexpr (XS) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[m][n][i] = acc[m][n][i];
     }
     if constexpr (GRAD) {
       const float down = 1.0f / a.norm[expert];  // a power of two, as are the rows' factors
