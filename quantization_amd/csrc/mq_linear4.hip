@@ -419,11 +419,11 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
   }
   // Tile height and cuts of the contraction (pieces of at least 4 blocks of 128, joined by a second launch): the cheapest
   // by what was measured on 4096 x 4096, microseconds per block of 128 for a compute unit with one tile (two sets of waves
-  // in it), with two, and for an odd one behind pairs.  64 x 128: 0.7, 1.55, 0.7 (gradient 1.5, 2.9, 1.5), 128 x 128:
-  // 1.2, 2.3, 1.3, the gradient's 128 x 256: 2.6, 5.0, 3.4 (it decodes half as often per product: 4096 rows 162 against 235
-  // with 128 x 128; one tile with one set of waves takes 3.4, pairs with two sets 5.6).  A tile begins and ends in 1.5; a
-  // join takes 3 and moves its sums at about 4 MB per microsecond.
-  static const double kTime[2][2][3] = {{{0.7, 1.55, 0.7}, {1.2, 2.3, 1.3}}, {{1.5, 2.9, 1.5}, {2.6, 5.0, 3.4}}};
+  // in it), with two, and for an odd one behind pairs.  64 x 128 (always two sets): 0.65, 1.3, 0.55 (gradient 0.85, 1.25,
+  // 0.65), 128 x 128: 1.15, 2.05, 1.1, the gradient's 128 x 256: 2.2, 3.8, 2.0 (one tile with one set of waves: forward
+  // 1.25, gradient 2.3; pairs with two sets: 2.35 and 4.3).  A tile begins and ends in 1.5; a join takes 3 and moves its
+  // sums at about 4 MB per microsecond.
+  static const double kTime[2][2][3] = {{{0.65, 1.3, 0.55}, {1.15, 2.05, 1.1}}, {{0.85, 1.25, 0.65}, {2.2, 3.8, 2.0}}};
   double best = 0;
   for (int tall = 0; tall < 2; ++tall) {
     const int bm = tall ? 128 : 64, bn = tall && grad ? 256 : 128;

@@ -214,10 +214,6 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_w4_rows(const W4A
 // integers is exact, the product rounds once (2^-11 of the weight at most).
 template <int KIND> struct W4Scales {
   u32x4 s, z;
-  __device__ __forceinline__ void load(const W4Product& p, int64_t at) {
-    s = *reinterpret_cast<const u32x4*>(p.ts + at);
-    if constexpr (KIND == W4_U4) z = *reinterpret_cast<const u32x4*>(p.tz + at);
-  }
   __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
     const u32x4 v = w4_decode<W4F16, KIND>(d, lut);
     // (whole vectors: the compiler takes a bit cast of one element of a vector for one of its first element)
@@ -267,9 +263,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
   constexpr int PAIRS = W == 4 ? 2 : 1;
   static_assert(BM / 4 % NW == 0 && BM % 64 == 0, "the rows of a block are dealt evenly");
   __shared__ u32x4 lds_all[WK][2][BM * 16];
+  constexpr int SETS = FS == 1 ? NT : 1;          // gradient: groups under a wave's 32 NT columns
+  constexpr int SZ = KIND == W4_U4 ? 2 : 1;       // scales, and zero points
+  __shared__ u32x4 lds_sc_all[GRAD ? WK * NW : 1][2][SETS][SZ][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int w = wave % NW, wk = wave / NW, wm = w % WM, wn = w / WM;
   auto& lds = lds_all[wk];
+  auto& lds_sc = lds_sc_all[GRAD ? wave : 0];  // of this wave alone
   // Workgroups go to the eight chiplets in turn: row tile 8 i + c belongs to chiplet c, whose L2 then holds its rows for all
   // columns; the row tiles behind the last eight are dealt out by columns.
   const uint32_t whole = (uint32_t)p.mblocks / 8 * (uint32_t)p.nblocks * 8, id = blockIdx.x;
@@ -313,17 +313,25 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       xo[c] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.ldx * 2u + (((lane & 15) ^ (r & 15)) * 16);
     }
     const int kb0 = (int)((int64_t)p.rb * blockIdx.y / p.splits), kb1 = (int)((int64_t)p.rb * (blockIdx.y + 1) / p.splits);
-    int64_t st0[NT];  // gradient: this lane's first scale under column tile n
+    int64_t st0[SETS];  // gradient: the wave's scales along the contraction, two to a lane
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int64_t c = tile0 + n, last = (p.ct - 1) >> 1;
-      st0[n] = ((int64_t)expert * a.gp + w4_group(a, (int)(c < last ? c : last))) * p.rb * 128 + half * 8;
+    for (int g = 0; g < SETS; ++g) {
+      const int64_t c = tile0 + g, last = (p.ct - 1) >> 1;
+      st0[g] = ((int64_t)expert * a.gp + w4_group(a, (int)(c < last ? c : last))) * p.rb * 128 + lane * 2;
     }
     W4Ahead<NT, GRAD ? 1 : W> next;
     auto fetch = [&](int kb, int buf, W4Ahead<NT, GRAD ? 1 : W>& to) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xsrc, (w4_lds_t*)&lds[buf][(w * CH + c) * 64], 16, xo[c], kb * 256, 0, 0);
+      if constexpr (GRAD) {
+#pragma unroll
+        for (int g = 0; g < SETS; ++g) {
+          __builtin_amdgcn_global_load_lds((w4_global_t*)(p.ts + st0[g] + kb * 128), (w4_lds_t*)lds_sc[buf][g][0], 4, 0, 0);
+          if constexpr (SZ == 2)
+            __builtin_amdgcn_global_load_lds((w4_global_t*)(p.tz + st0[g] + kb * 128), (w4_lds_t*)lds_sc[buf][g][SZ - 1], 4, 0, 0);
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -343,11 +351,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       if (kb + WK < kb1) fetch(kb + WK, buf ^ 1, next);
       const u32x4* xb = lds[buf] + (wm * MT * 32 + l32) * 16;
       const int turn = (l32 & 15) ^ half;
-      // One row tile: its operands of the whole block at once, since two products hide no LDS load.
-      u32x4 xa[MT == 1 ? 8 : 1];
-      if constexpr (MT == 1) {
+      // Two products to a step hide no LDS load: the operands of the whole block at once.
+      constexpr bool ALL = MT * NT <= 2;
+      u32x4 xa[ALL ? MT : 1][ALL ? 8 : 1];
+      if constexpr (ALL) {
 #pragma unroll
-        for (int st = 0; st < 8; ++st) xa[st] = xb[(2 * st) ^ turn];
+        for (int st = 0; st < 8; ++st)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) xa[m][st] = xb[m * 512 + ((2 * st) ^ turn)];
       }
       if (WK > 1 && kb >= kb1) {
         // the other waves' last block: nothing for this half
@@ -380,7 +391,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
         for (int st = 0; st < 8; ++st) {
           u32x4 xv[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) xv[m] = MT == 1 ? xa[MT == 1 ? st : 0] : xb[m * 512 + ((2 * st) ^ turn)];
+          for (int m = 0; m < MT; ++m) xv[m] = ALL ? xa[ALL ? m : 0][ALL ? st : 0] : xb[m * 512 + ((2 * st) ^ turn)];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const u32x4 v = w4_decode<T, KIND>(cur.b[n][st & 1][st >> 1], a.lut);
@@ -421,15 +432,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
           }
         }
       } else {
-        constexpr int SETS = FS == 1 ? NT : 1;  // groups under a wave's 32 NT columns
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
           W4Scales<KIND> sc[SETS];
 #pragma unroll
-          for (int g = 0; g < SETS; ++g) sc[g].load(p, st0[g] + kb * 128 + st * 16);
+          for (int g = 0; g < SETS; ++g) {
+            sc[g].s = lds_sc[buf][g][0][st * 2 + half];
+            if constexpr (SZ == 2) sc[g].z = lds_sc[buf][g][SZ - 1][st * 2 + half];
+          }
           u32x4 xv[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) xv[m] = MT == 1 ? xa[MT == 1 ? st : 0] : xb[m * 512 + ((2 * st) ^ turn)];
+          for (int m = 0; m < MT; ++m) xv[m] = ALL ? xa[ALL ? m : 0][ALL ? st : 0] : xb[m * 512 + ((2 * st) ^ turn)];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const u32x4 v = sc[FS == 1 ? n : 0].scaled(cur.b[n][st & 1][st >> 1], a.lut);
@@ -595,13 +608,13 @@ hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool
     else if (pl.nt == 2) w4_rows_go<T, KIND, 2, 2>(a, p, pl, st);
     else w4_rows_go<T, KIND, 2, 4>(a, p, pl, st);
   } else if (grad) {
-    if (pl.bm == 64) w4_gemm_go<W4F16, T, KIND, true, 1, 2, 2, 2, 2>(a, p, pl, st);
+    if (pl.bm == 64) w4_gemm_go<W4F16, T, KIND, true, 2, 1, 1, 4, 2>(a, p, pl, st);
     else if (pl.wk == 2) w4_gemm_go<W4F16, T, KIND, true, 4, 2, 1, 4, 2>(a, p, pl, st);
     else w4_gemm_go<W4F16, T, KIND, true, 4, 2, 1, 4, 1>(a, p, pl, st);
   } else {
-    if (pl.bm == 64) w4_gemm_go<T, T, KIND, false, 1, 2, 2, 2, 2>(a, p, pl, st);
+    if (pl.bm == 64) w4_gemm_go<T, T, KIND, false, 2, 1, 1, 4, 2>(a, p, pl, st);
     else if (pl.wk == 2) w4_gemm_go<T, T, KIND, false, 2, 2, 2, 2, 2>(a, p, pl, st);
-    else w4_gemm_go<T, T, KIND, false, 2, 2, 2, 2, 1>(a, p, pl, st);
+    else w4_gemm_go<T, T, KIND, false, 4, 1, 1, 4, 1>(a, p, pl, st);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.part) return e;
