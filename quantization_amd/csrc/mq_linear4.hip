@@ -39,7 +39,7 @@ struct PackArgs {
 };
 
 // One thread per dword: eight codes of one row.  Consecutive threads take consecutive octets of a row, so that a wave
-// reads four rows' 128 bytes each.
+// reads four rows' 128 bytes each.  Runs once per weight; its byte loads bound it (14336 x 4096: 39 us, 2.3 TB/s).
 template <int KIND> __global__ __launch_bounds__(256) void k_w4_pack(const PackArgs p) {
   const int t = threadIdx.x, octet = t & 15, r = t >> 4;
   const int64_t n = (int64_t)blockIdx.y * 16 + r, k0 = (int64_t)blockIdx.x * 128 + octet * 8;
@@ -84,7 +84,8 @@ __global__ __launch_bounds__(256) void k_w4_params(const PackArgs p, int64_t tot
   }
 }
 
-// The float16 weight: h(h(q - zero) * scale), the arithmetic of the quantizers' dequantization.
+// The float16 weight: h(h(q - zero) * scale), the arithmetic of the quantizers' dequantization, eight values to a thread.
+// Bound by its bytes.
 template <int KIND> __global__ __launch_bounds__(256) void k_w4_unpack(const W4Args a, uint16_t* out) {
   const int t = threadIdx.x, octet = t & 15, r = t >> 4;
   const int64_t n = (int64_t)blockIdx.y * 16 + r, k0 = (int64_t)blockIdx.x * 128 + octet * 8, e = blockIdx.z;
@@ -102,15 +103,26 @@ template <int KIND> __global__ __launch_bounds__(256) void k_w4_unpack(const W4A
   } else {
     s = (float)h_from_bits(static_cast<const uint16_t*>(a.params)[at]);
   }
-  for (int i = 0; i < 8 && k0 + i < a.k; ++i) {
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
     float q = f[i];
     if constexpr (KIND == W4_U4) q = (float)h_from_bits(f2h_bits(q - z));
-    out[(e * a.n + n) * a.k + k0 + i] = (uint16_t)f2h_bits(q * s);
+    h[i] = f2h_bits(q * s) & 0xFFFFu;
+  }
+  uint16_t* to = out + (e * a.n + n) * a.k + k0;
+  if (a.k % 8 == 0 && (uintptr_t)out % 16 == 0) {
+    *reinterpret_cast<u32x4*>(to) = u32x4{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i < a.k) to[i] = (uint16_t)h[i];
   }
 }
 
 // ---- rows that the products cannot read as they are -------------------------------------------------
-// Rows of any stride, alignment and length -> rows of 128 rb elements, zeros behind the end.
+// Rows of any stride, alignment and length -> rows of 128 rb elements, zeros behind the end.  A copy before the products
+// keeps the bounds of rows out of their loops; its element loads bound it (2048 rows of 4096 at an odd address: 12 us, 2.7 TB/s).
 __global__ __launch_bounds__(256) void k_w4_pad(const W4Product p, int64_t rows, uint16_t* to) {
   const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), k = (int64_t)blockIdx.y * 128 + (threadIdx.x & 15) * 8;
   if (r < rows) *reinterpret_cast<u32x4*>(to + r * p.rb * 128 + k) = w4_load8(p.x + r * p.ldx, k, p.kc, p.vec);
@@ -119,7 +131,8 @@ __global__ __launch_bounds__(256) void k_w4_pad(const W4Product p, int64_t rows,
 // Rows of bfloat16 -> rows of float16 times a power of two each, which brings a row's largest value into [2^14, 2^15):
 // eight significant bits fit float16's eleven, so nothing is lost but of values more than 2^28 below the largest.
 // down[row]: the inverse factor.  A row that holds an infinity or NaN keeps its scale (its results are not finite anyway).
-// One wave to a row; the second pass finds the row in the caches.
+// One wave to a row; the second pass finds the row in the caches.  It shares k_w4_turn's launch, which leaves compute units
+// free: 2048 rows of 4096 beside the turning of 4096 x 4096 take 11.4 us, the turning alone 7.7.
 __device__ __forceinline__ void w4_half_row(const W4Product& p, int64_t row, uint16_t* to, float* down) {
   const int lane = threadIdx.x & 63;
   const uint16_t* from = p.x + row * p.ldx;
@@ -158,7 +171,9 @@ __device__ __forceinline__ void w4_half_row(const W4Product& p, int64_t row, uin
 // exchanged.  A wave turns 128 rows x 128 columns, a thread 8 rows x 32 columns: it
 // reads four dwords of each row at once (8 x 16 contiguous bytes) and turns four blocks of 8 x 8 nibbles in registers, by
 // exchanging nibbles, bytes and halves between pairs of dwords (32 instructions a block).  The turned dwords go through
-// LDS, so that whole tiles are stored.  Bound by its bytes: half a byte read and written per weight.
+// LDS, so that whole tiles are stored.  Bound by its bytes, half a byte read and written per weight: 32 experts of
+// 2048 x 2048 (134 MB) with 4096 rows of bfloat16 beside them 36 us, 3.7 TB/s.  One wave to a workgroup: nobody waits for
+// another's loads.
 // It also writes the scales (and zero points) along the contraction, in the form that W4Scales loads.
 struct TurnArgs {
   uint32_t* out;  // [E][ct][rb][64][4]
@@ -268,7 +283,8 @@ template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args
 
 // ---- the bias's gradient -----------------------------------------------------------------------------
 // Sums of dy's rows per expert in float32: 64 columns to a workgroup, whose sixteen waves take the rows in turn; where an
-// expert has many rows they are cut into runs, whose sums a second launch adds in order.  Bound by reading dy once more.
+// expert has many rows they are cut into runs, whose sums a second launch adds in order.  Bound by reading dy once more,
+// which the caches mostly hold, and by a launch (509 x 2048: 5.4 us).  No atomics: the order of the sum is fixed.
 struct BiasArgs {
   const uint16_t* dy;
   const int32_t* counts;
@@ -419,11 +435,11 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
   }
   // Tile height and cuts of the contraction (pieces of at least 4 blocks of 128, joined by a second launch): the cheapest
   // by what was measured on 4096 x 4096, microseconds per block of 128 for a compute unit with one tile (two sets of waves
-  // in it), with two, and for an odd one behind pairs.  64 x 128 (always two sets): 0.65, 1.3, 0.55 (gradient 0.85, 1.25,
-  // 0.65), 128 x 128: 1.15, 2.05, 1.1, the gradient's 128 x 256: 2.2, 3.8, 2.0 (one tile with one set of waves: forward
-  // 1.25, gradient 2.3; pairs with two sets: 2.35 and 4.3).  A tile begins and ends in 1.5; a join takes 3 and moves its
+  // in it), with two, and for an odd one behind pairs.  64 x 128 (always two sets): 0.65, 1.3, 0.55 (gradient 0.85, 1.2,
+  // 0.65), 128 x 128: 1.05, 1.85, 1.2, the gradient's 128 x 256: 2.15, 3.75, 1.8 (one tile with one set of waves: forward
+  // 1.1, gradient 2.3; pairs with two sets: 2.15 and 4.15).  A tile begins and ends in 1.5; a join takes 3 and moves its
   // sums at about 4 MB per microsecond.
-  static const double kTime[2][2][3] = {{{0.65, 1.3, 0.55}, {1.15, 2.05, 1.1}}, {{0.85, 1.25, 0.65}, {2.2, 3.8, 2.0}}};
+  static const double kTime[2][2][3] = {{{0.65, 1.3, 0.55}, {1.05, 1.85, 1.2}}, {{0.85, 1.2, 0.65}, {2.15, 3.75, 1.8}}};
   double best = 0;
   for (int tall = 0; tall < 2; ++tall) {
     const int bm = tall ? 128 : 64, bn = tall && grad ? 256 : 128;

@@ -79,8 +79,6 @@ template <int KIND> constexpr float w4_byte_scale() { return KIND == W4_U4 || KI
 
 struct W4F16 {  // element traits: float16
   static constexpr bool kHalf = true;
-  typedef _Float16 elem;
-  typedef w4_h8 vec8;
   template <bool HI> static __device__ __forceinline__ uint32_t from_fp8(uint32_t v, float s) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, s, HI));
   }
@@ -105,8 +103,6 @@ struct W4F16 {  // element traits: float16
 };
 struct W4BF16 {  // element traits: bfloat16
   static constexpr bool kHalf = false;
-  typedef __bf16 elem;
-  typedef w4_b8 vec8;
   template <bool HI> static __device__ __forceinline__ uint32_t from_fp8(uint32_t v, float s) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, s, HI));
   }
@@ -189,7 +185,7 @@ struct W4Args {
 // (2 s + 1) * 2 gu <= 2^32, and s, gu < 2^15 (columns <= 2^20).
 __device__ __forceinline__ int w4_group(const W4Args& a, int step) { return (int)__umulhi((uint32_t)(2 * step + 1), a.gmagic); }
 
-// Inclusive sum over the lanes of a wave, cut off at `top` (0 <= v <= top < 2^30), in the vector unit's own lane moves.
+// Inclusive sum over the lanes of a wave, cut off at `top` (0 <= v <= top < 2^31), in the vector unit's own lane moves.
 __device__ __forceinline__ uint32_t w4_scan(uint32_t v, uint32_t top) {
 #define MQ_W4_SCAN_STEP(CTRL, ROWS)                                                             \
   {                                                                                             \

@@ -13,7 +13,7 @@ struct W4Product {
   float* xs;             // sums of x per window and row (k_w4_rowsum), for zero points in k_w4_gemm
   const uint16_t* ts;    // gradient: scales along the contraction times norm, k_w4_turn's [E][GP][128 rb]
   const uint16_t* tz;    // ... and zero points
-  const float* down;     // gradient of bfloat16: what k_w4_half's rows have to be multiplied by
+  const float* down;     // gradient of bfloat16: what w4_half_row's rows have to be multiplied by
   int64_t ldx, kc, nc;   // contraction length, output columns
   int32_t ct, rb;        // 16-column tiles of the output, 128-blocks of the contraction
   int32_t vec;           // rows of x are 16-byte aligned and kc % 8 == 0
@@ -49,10 +49,14 @@ template <class T> __device__ __forceinline__ void w4_store4(uint16_t* y, int64_
   }
 }
 // ---- few rows --------------------------------------------------------------------------------------
-// A workgroup owns NT column tiles and 16 * MT rows; its waves take the 128-blocks of the contraction in turn and their
-// sums meet in LDS at the end, in the waves' order.  Everything is in registers on its way: a wave keeps D blocks in
-// flight while it works on the D before them.  Rows that are not there repeat the tile's last one (their loads fall into
-// the same lines, their results are not stored; masking them off measured slower).  Rows are 16-byte aligned and a multiple of 128 long (k_w4_pad).
+// y = sum over groups of scale * (sum q x - zero sum x), in tiles of v_mfma_f32_16x16x32 with x as the A operand; the sums
+// of x are a product with ones.  A workgroup owns NT column tiles and 16 * MT rows; its waves take the 128-blocks of the
+// contraction in turn and their sums meet in LDS at the end, in the waves' order.  Everything is in registers on its way: a
+// wave keeps D blocks in flight while it works on the D before them.  Rows that are not there repeat the tile's last one
+// (their loads fall into the same lines, their results are not stored; masking them off measured slower).  Rows are 16-byte
+// aligned and a multiple of 128 long (k_w4_pad).
+// Bound by reading the weight: 5 rows through 128256 x 4096 (280 MB) 48 us, 5.8 TB/s; one row through 14336 x 4096 with
+// zero points (31 MB) 9.0 us, 3.5 TB/s; 2048 x 2048 3.9 us, which is the latency of a launch and of two blocks.
 template <class T, int KIND, int MT, int NT, int FS, int D> struct W4RowsStage {
   u32x4 w[D][NT], x[D][MT][4];
   uint32_t s[D][NT];  // lane 16 v + c: the scale (and zero point) of column c in window v of the block's 4 / FS
@@ -210,8 +214,9 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_w4_rows(const W4A
 }
 
 // ---- the gradient's scaled weights ---------------------------------------------------------------------
-// Eight weights of one column in float16, scale * (q - zero) times the expert's norm (a power of two): the difference of
-// integers is exact, the product rounds once (2^-11 of the weight at most).
+// Eight weights of one column in float16, scale * (q - zero) times the expert's norm (a power of two): the difference is
+// exact for zero points up to 2033 (beyond it rounds as the quantizers' dequantization does), the product rounds once (2^-11
+// of the weight at most).
 template <int KIND> struct W4Scales {
   u32x4 s, z;
   __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
@@ -230,18 +235,31 @@ template <int KIND> struct W4Scales {
 // 256 bytes a row, its sixteen 16-byte pieces permuted by the row (piece c stands at c ^ (row % 16)), so that rows are
 // fetched in whole lines and neither the writes nor the operand reads meet in a bank.  The packed weight goes from memory
 // straight into the registers of the wave that decodes it: lane l takes row l % 32 of the 32-row tile, the halves of its
-// wave the eight columns 8 (l / 32) of every sixteen -- two of the layout's four dwords-quadruples.
-// WK = 2: two sets of waves with buffers of their own take the blocks of the contraction in turn, for small tiles and where
-// a compute unit has only one: one wave per SIMD would wait for its own decoding.
+// wave the eight columns 8 (l / 32) of every sixteen -- two of the layout's four dwords-quadruples.  Waves stand side by
+// side along the columns (WM = 1): no two of them decode the same weights, at the price of reading all rows from LDS each
+// (384 rows, 4096 x 14336 with zero points: 91 us, 105 with two by two waves).
+// WK = 2: two sets of waves with buffers of their own take the blocks of the contraction in turn, for tiles of 64 rows and
+// where a compute unit has only one tile: one wave per SIMD would wait for its own decoding.  Four sets gave nothing more.
 // Rows are 16-byte aligned and a multiple of 128 long here: others are copied first (k_w4_pad).
-// GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.  Zero
-// points: minus (scale * zero)[column] * (sum of x)[row] per window of FS steps, a float32 product on the matrix cores
-// with a contraction over the windows (v_mfma_f32_32x32x2_f32): done by the vector units it took as many instructions
-// again as the scaling.
+//
+// GRAD = false: sums run over exact code values; every FS steps of 32 they are scaled in float32 into the result.  The row
+// tiles are taken in two halves, first with the decoding, then with the decoded operands once more, and the scaling of one
+// half is dealt out between the products of the other: in one piece it left the matrix cores idle (2000 x 14336 x 4096:
+// 232 us).  The second half has the higher priority in the SIMD, so that its products run while another wave decodes (223
+// to 218).  Zero points: minus (scale * zero)[column] * (sum of x)[row] per window of FS steps, a float32 product on the
+// matrix cores with a contraction over the windows (v_mfma_f32_32x32x2_f32): the vector units took as many instructions
+// for it as for the scaling (2048 x 4096 x 4096, groups of 64: 106 us, 100 with the product).
+// 2000 rows through 14336 x 4096: 218 us, 1.08 PFLOP/s.  The matrix cores are busy in 0.59 of the cycles, 168 vector
+// instructions stand beside every 32 products, and under this load the clock falls to 1.8 GHz: the steps above took 11 % of
+// the cycles away and 4 % of the time.
+//
 // GRAD = true (dx = dy W, operand b transposed): scales change along the contraction, so they are multiplied into the
 // weights, which are rounded once to float16 (W4Scales).  It runs in float16 for both types: rows of bfloat16 are brought
-// into its range by a power of two each (k_w4_half), where they lose nothing, while weights rounded to bfloat16 would add
-// as much error as the rounding of the result (2.4e-3 of the norm against 1.7e-3) and take more instructions to make.
+// into its range by a power of two each (w4_half_row), where they lose nothing, while weights rounded to bfloat16 would add
+// as much error as the rounding of the result (2.4e-3 of the norm against 1.7e-3) and take more instructions to make.  The
+// scales along the contraction come with the block's rows through LDS, two to a lane (4096 x 4096 x 4096: 137 us, 149 with
+// loads between the products).  2048 rows through 4096 x 4096, one tile to a compute unit: 89 us with zero points, the matrix
+// cores busy in 0.33 of the cycles, the waves waiting for loads in 0.38; 4096 rows: 1.03 PFLOP/s, turning included.
 template <int NT, int W> struct W4Ahead {  // what a wave holds of a block that is on its way
   u32x4 b[NT][2];
   uint32_t s[NT][W];
@@ -281,7 +299,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
   int64_t row0;
   if (!w4_find_tile(a, BM, mb, expert, row0, rows)) return;
   f32x16 acc[MT][NT];     // GRAD, zero points: the matrix instructions' own sums
-  float sum[MT][NT][16];  // forward: the scaled sums (single registers: they are never a matrix operand)
+  float sum[MT][NT][16];  // forward: the scaled sums (single registers, where they are no matrix operand)
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -343,6 +361,31 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
         }
       }
     };
+    // forward: the row tiles' halves.  `hi` holds the second half's unscaled sums until the next window's first products,
+    // sh their scales.
+    constexpr int MH = MT / 2;
+    static_assert(GRAD || MT % 2 == 0, "two halves");
+    f32x16 hi[GRAD ? 1 : MH][NT];
+    float sh[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      sh[n] = 0;
+#pragma unroll
+      for (int m = 0; m < (GRAD ? 1 : MH); ++m) hi[m][n] = w4_zero16();
+    }
+    // the share of product step `step` in scaling a half's sums: none behind the first step, while they are on their way
+    auto add = [&](const f32x16 (&from)[GRAD ? 1 : MH][NT], const float (&by)[NT], int m0, int step) {
+      constexpr int ALL = MH * NT * 16, S = 2 * FS - 1;
+#pragma unroll
+      for (int i = 0; i < ALL; ++i) {
+        if (step == 0 || i < ALL * (step - 1) / S || i >= ALL * step / S) continue;
+        const int m = i / (16 * NT), n = i / 16 % NT, r = i % 16;
+        if constexpr (XS)
+          acc[m0 + m][n][r] = __builtin_fmaf(by[n], from[m][n][r], acc[m0 + m][n][r]);
+        else
+          sum[m0 + m][n][r] = __builtin_fmaf(by[n], from[m][n][r], sum[m0 + m][n][r]);
+      }
+    };
     if (kb0 + wk < kb1) fetch(kb0 + wk, 0, next);
     __syncthreads();
     for (int it = 0; kb0 + it * WK < kb1; ++it) {
@@ -351,15 +394,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       if (kb + WK < kb1) fetch(kb + WK, buf ^ 1, next);
       const u32x4* xb = lds[buf] + (wm * MT * 32 + l32) * 16;
       const int turn = (l32 & 15) ^ half;
-      // Two products to a step hide no LDS load: the operands of the whole block at once.
-      constexpr bool ALL = MT * NT <= 2;
-      u32x4 xa[ALL ? MT : 1][ALL ? 8 : 1];
-      if constexpr (ALL) {
-#pragma unroll
-        for (int st = 0; st < 8; ++st)
-#pragma unroll
-          for (int m = 0; m < MT; ++m) xa[m][st] = xb[m * 512 + ((2 * st) ^ turn)];
-      }
       if (WK > 1 && kb >= kb1) {
         // the other waves' last block: nothing for this half
       } else if constexpr (!GRAD) {
@@ -386,40 +420,57 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
             }
           }
         }
-        f32x16 tmp[MT][NT];
+        f32x16 lo[MH][NT];
+        u32x4 xv[2][MH];
+        // operands of product step t = 4 FS window + 2 FS half + step, read from LDS a step ahead
+        auto rows_of = [&](int t) {
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {
-          u32x4 xv[MT];
+          for (int m = 0; m < MH; ++m) {
+            const int st = t / (4 * FS) * 2 * FS + t % (2 * FS), first = t / (2 * FS) % 2 * MH;
+            if (t < 16) xv[t & 1][m] = xb[(first + m) * 512 + ((2 * st) ^ turn)];
+          }
+        };
+        rows_of(0);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) xv[m] = ALL ? xa[ALL ? m : 0][ALL ? st : 0] : xb[m * 512 + ((2 * st) ^ turn)];
+        for (int v = 0; v < W; ++v) {
+          float s[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const u32x4 v = w4_decode<T, KIND>(cur.b[n][st & 1][st >> 1], a.lut);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) tmp[m][n] = T::mfma32(xv[m], v, st % (2 * FS) == 0 ? w4_zero16() : tmp[m][n]);
+            s[n] = (float)h_from_bits(cur.s[n][v]);
+            asm("" : "+v"(s[n]));  // a float32 register: v_fmac_f32 issues faster than the mixed fma the compiler would choose
           }
-          if ((st + 1) % (2 * FS) == 0) {
-            const int v = st / (2 * FS);
-            float s[NT];
+          // (each step is fixed in its place: left alone, the scheduler gathers the scaling behind the products)
+          u32x4 q[2 * FS][NT];
+#pragma unroll
+          for (int i = 0; i < 2 * FS; ++i) {  // the first half of the row tiles; the second's sums of the window before
+            const int st = v * 2 * FS + i, t = v * 4 * FS + i;
+            rows_of(t + 1);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              s[n] = (float)h_from_bits(cur.s[n][v]);
-              asm("" : "+v"(s[n]));  // a float32 register: v_fmac_f32 issues faster than the mixed fma the compiler would choose
+              q[i][n] = w4_decode<T, KIND>(cur.b[n][st & 1][st >> 1], a.lut);
+#pragma unroll
+              for (int m = 0; m < MH; ++m)
+                lo[m][n] = T::mfma32(xv[t & 1][m], q[i][n], i == 0 ? w4_zero16() : lo[m][n]);
             }
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  if constexpr (XS)
-                    acc[m][n][i] = __builtin_fmaf(s[n], tmp[m][n][i], acc[m][n][i]);
-                  else
-                    sum[m][n][i] = __builtin_fmaf(s[n], tmp[m][n][i], sum[m][n][i]);
-                }
-            // one window's unscaled sums at a time: without this the scheduler keeps several in registers and spills
-            if (FS < 4) __builtin_amdgcn_sched_barrier(0);
+            add(hi, sh, MH, i);
+            __builtin_amdgcn_sched_barrier(0);
           }
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int i = 0; i < 2 * FS; ++i) {
+            const int t = v * 4 * FS + 2 * FS + i;
+            rows_of(t + 1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int m = 0; m < MH; ++m)
+                hi[m][n] = T::mfma32(xv[t & 1][m], q[i][n], i == 0 ? w4_zero16() : hi[m][n]);
+            add(lo, s, 0, i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) sh[n] = s[n];
         }
         if constexpr (XS) {
           if (pair_now) {
@@ -432,6 +483,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
           }
         }
       } else {
+        // Two products to a step hide no LDS load: the operands of the whole block at once.
+        constexpr bool ALL = MT * NT <= 2;
+        u32x4 xa[ALL ? MT : 1][ALL ? 8 : 1];
+        if constexpr (ALL) {
+#pragma unroll
+          for (int st = 0; st < 8; ++st)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xa[m][st] = xb[m * 512 + ((2 * st) ^ turn)];
+        }
 #pragma unroll
         for (int st = 0; st < 8; ++st) {
           W4Scales<KIND> sc[SETS];
@@ -452,6 +512,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
         }
       }
       __syncthreads();
+    }
+    if constexpr (!GRAD) {
+#pragma unroll
+      for (int i = 1; i < 2 * FS; ++i) add(hi, sh, MH, i);
     }
     if constexpr (XS) {
 #pragma unroll
@@ -512,7 +576,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       for (int i = 0; i < 16; i += 2) {
         const bool odd = lane & 1;
         const float mine = odd ? sum[m][n][i + 1] : sum[m][n][i], other = odd ? sum[m][n][i] : sum[m][n][i + 1];
-        const float got = __shfl_xor(other, 1);
+        const float got = f_from_bits((uint32_t)__builtin_amdgcn_mov_dpp((int)__builtin_bit_cast(uint32_t, other), 0xB1, 0xF, 0xF, true));  // lane ^ 1
         const float v0 = (odd ? got : mine) + b0, v1 = (odd ? mine : got) + b1;
         const int r = (wm * MT + m) * 32 + (i >> 2) * 8 + half * 4 + (i & 3) + odd;
         if (r < rows && col < p.nc) {
@@ -536,7 +600,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
 }
 
 // Sums of x over the windows of 32 FS columns that k_w4_gemm scales at a time: xs[window][row], for the zero points.
-// A wave takes four rows x 128 columns.
+// A wave takes four rows x 128 columns.  Bound by reading x (2048 x 4096, 16 MB: 5.4 us, 3.1 TB/s); every column tile of
+// the product would have to add them up again.
 template <class T, int FS> __global__ __launch_bounds__(256) void k_w4_rowsum(const W4Product p, int64_t rows, float* xs) {
   const int lane = threadIdx.x & 63;
   const int64_t r = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4);
@@ -550,7 +615,8 @@ template <class T, int FS> __global__ __launch_bounds__(256) void k_w4_rowsum(co
   if (r < rows && (lane & (4 * FS - 1)) == 0) xs[((int64_t)kb * (4 / FS) + (lane & 15) / (4 * FS)) * rows + r] = s;
 }
 
-// The splits' partial sums, added in their order.
+// The splits' partial sums, added in their order.  Bound by a launch and by the sums' bytes, which the caches hold (77 x
+// 5632, two splits, 3.5 MB: 4 us of which the launch is 2).
 template <class T> __global__ __launch_bounds__(256) void k_w4_join(const W4Product p, int64_t rows) {
   const int64_t quads = (int64_t)p.ct * 4, total = rows * quads;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -613,7 +679,7 @@ hipError_t w4_launch(const W4Args& a, const W4Product& p, const W4Plan& pl, bool
     else w4_gemm_go<W4F16, T, KIND, true, 4, 2, 1, 4, 1>(a, p, pl, st);
   } else {
     if (pl.bm == 64) w4_gemm_go<T, T, KIND, false, 2, 1, 1, 4, 2>(a, p, pl, st);
-    else if (pl.wk == 2) w4_gemm_go<T, T, KIND, false, 2, 2, 2, 2, 2>(a, p, pl, st);
+    else if (pl.wk == 2) w4_gemm_go<T, T, KIND, false, 4, 1, 1, 4, 2>(a, p, pl, st);
     else w4_gemm_go<T, T, KIND, false, 4, 1, 1, 4, 1>(a, p, pl, st);
   }
   hipError_t e = hipGetLastError();
