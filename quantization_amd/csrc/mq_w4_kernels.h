@@ -215,7 +215,7 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_w4_rows(const W4A
 
 // ---- the gradient's scaled weights ---------------------------------------------------------------------
 // Eight weights of one column in float16, scale * (q - zero) times the expert's norm (a power of two): the difference is
-// exact for zero points up to 2033 (beyond it rounds as the quantizers' dequantization does), the product rounds once (2^-11
+// exact for zero points up to 2048 (beyond it rounds as the quantizers' dequantization does), the product rounds once (2^-11
 // of the weight at most).
 template <int KIND> struct W4Scales {
   u32x4 s, z;

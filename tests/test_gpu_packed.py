@@ -107,6 +107,31 @@ def test_linear_many_rows_with_bias(pk, fmt, bits, dtype):
             near(pk.packed_linear(x, p, b), product(x, w) + b.double(), product(x.abs(), mass) + b.double().abs(), k, p, what=(n, k, g, m))
 
 
+@pytest.mark.parametrize("g", [32, 64, 128, 256, None])
+@pytest.mark.parametrize("fmt", ["int4", "int4_asym"])
+def test_every_number_of_blocks(pk, fmt, g):
+    """Contractions of one to nine blocks of 128 (windows of zero points in pairs, blocks in two wave sets, cuts) under each
+    tile: few rows, one tile to a compute unit, several."""
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    for blocks in range(1, 10):
+        k = blocks * 128
+        if g and k % g:
+            continue
+        p, w, mass, _ = weight(gen, (1100, k), fmt, 4, g)
+        for dtype, m in ((torch.float16, 47), (torch.bfloat16, 200), (torch.float16, 1300), (torch.bfloat16, 4200)):
+            x = torch.randn(m, k, generator=gen, device="cuda").to(dtype)
+            near(pk.packed_linear(x, p), product(x, w), product(x.abs(), mass), k, p, what=(blocks, m))
+    # the gradient: the same along the weight's rows
+    for blocks in range(1, 10):
+        n = blocks * 128 - blocks % 3
+        p, w, mass, _ = weight(gen, (n, 1280), fmt, 4, g)
+        for dtype, m in ((torch.float16, 47), (torch.bfloat16, 200), (torch.float16, 1300), (torch.bfloat16, 8300)):
+            x = torch.zeros(m, 1280, device="cuda", dtype=dtype, requires_grad=True)
+            dy = torch.randn(m, n, generator=gen, device="cuda").to(dtype)
+            pk.packed_linear(x, p).backward(dy)
+            near(x.grad, dy.double() @ w, dy.double().abs() @ mass, n, p, rounded=True, what=("grad", blocks, m))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("fmt,bits", FORMATS)
 def test_linear_backward(pk, fmt, bits, dtype):
