@@ -264,7 +264,6 @@ template <int NT, int W> struct W4Ahead {  // what a wave holds of a block that 
   u32x4 b[NT][2];
   uint32_t s[NT][W];
 };
-typedef __attribute__((address_space(1))) const void w4_global_t;
 #ifdef __HIP_DEVICE_COMPILE__
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_buffer(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);  // raw 32-bit data
@@ -280,14 +279,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
   constexpr bool XS = KIND == W4_U4 && !GRAD;                       // zero points, taken away through the rows' sums
   constexpr int PAIRS = W == 4 ? 2 : 1;
   static_assert(BM / 4 % NW == 0 && BM % 64 == 0, "the rows of a block are dealt evenly");
-  __shared__ u32x4 lds_all[WK][2][BM * 16];
   constexpr int SETS = FS == 1 ? NT : 1;          // gradient: groups under a wave's 32 NT columns
   constexpr int SZ = KIND == W4_U4 ? 2 : 1;       // scales, and zero points
-  __shared__ u32x4 lds_sc_all[GRAD ? WK * NW : 1][2][SETS][SZ][16];
+  // One array for the rows' blocks [WK][2][BM * 16] and the gradient's scales [WK * NW][2][SETS][SZ][16]: of two arrays the
+  // compiler would order every read behind all loads on their way into LDS, those of the other buffer among them.
+  constexpr int ROWS = WK * 2 * BM * 16, SCALES = GRAD ? WK * NW * 2 * SETS * SZ * 16 : 0;
+  __shared__ u32x4 lds_all[ROWS + SCALES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int w = wave % NW, wk = wave / NW, wm = w % WM, wn = w / WM;
-  auto& lds = lds_all[wk];
-  auto& lds_sc = lds_sc_all[GRAD ? wave : 0];  // of this wave alone
+  u32x4* const lds = lds_all + wk * 2 * BM * 16;
+  u32x4* const lds_sc = lds_all + ROWS + wave * 2 * SETS * SZ * 16;  // of this wave alone
   // Workgroups go to the eight chiplets in turn: row tile 8 i + c belongs to chiplet c, whose L2 then holds its rows for all
   // columns; the row tiles behind the last eight are dealt out by columns.
   const uint32_t whole = (uint32_t)p.mblocks / 8 * (uint32_t)p.nblocks * 8, id = blockIdx.x;
@@ -331,23 +332,28 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       xo[c] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)p.ldx * 2u + (((lane & 15) ^ (r & 15)) * 16);
     }
     const int kb0 = (int)((int64_t)p.rb * blockIdx.y / p.splits), kb1 = (int)((int64_t)p.rb * (blockIdx.y + 1) / p.splits);
-    int64_t st0[SETS];  // gradient: the wave's scales along the contraction, two to a lane
+    // gradient: the wave's scales (and zero points) along the contraction, two to a lane
+    __amdgpu_buffer_rsrc_t ssrc[GRAD ? SETS : 1][SZ];
+    if constexpr (GRAD) {
 #pragma unroll
-    for (int g = 0; g < SETS; ++g) {
-      const int64_t c = tile0 + g, last = (p.ct - 1) >> 1;
-      st0[g] = ((int64_t)expert * a.gp + w4_group(a, (int)(c < last ? c : last))) * p.rb * 128 + lane * 2;
+      for (int g = 0; g < SETS; ++g) {
+        const int64_t c = tile0 + g, last = (p.ct - 1) >> 1;
+        const int64_t from = ((int64_t)expert * a.gp + w4_group(a, (int)(c < last ? c : last))) * p.rb * 128;
+        ssrc[g][0] = w4_buffer(p.ts + from, (uint32_t)p.rb * 256u);
+        if constexpr (SZ == 2) ssrc[g][SZ - 1] = w4_buffer(p.tz + from, (uint32_t)p.rb * 256u);
+      }
     }
     W4Ahead<NT, GRAD ? 1 : W> next;
     auto fetch = [&](int kb, int buf, W4Ahead<NT, GRAD ? 1 : W>& to) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xsrc, (w4_lds_t*)&lds[buf][(w * CH + c) * 64], 16, xo[c], kb * 256, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xsrc, (w4_lds_t*)(lds + buf * BM * 16 + (w * CH + c) * 64), 16, xo[c], kb * 256, 0, 0);
       if constexpr (GRAD) {
 #pragma unroll
         for (int g = 0; g < SETS; ++g) {
-          __builtin_amdgcn_global_load_lds((w4_global_t*)(p.ts + st0[g] + kb * 128), (w4_lds_t*)lds_sc[buf][g][0], 4, 0, 0);
-          if constexpr (SZ == 2)
-            __builtin_amdgcn_global_load_lds((w4_global_t*)(p.tz + st0[g] + kb * 128), (w4_lds_t*)lds_sc[buf][g][SZ - 1], 4, 0, 0);
+#pragma unroll
+          for (int z = 0; z < SZ; ++z)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ssrc[g][z], (w4_lds_t*)(lds_sc + ((buf * SETS + g) * SZ + z) * 16), 4, lane * 4, kb * 256, 0, 0);
         }
       }
 #pragma unroll
@@ -392,32 +398,40 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
       const int kb = kb0 + it * WK + wk, buf = it & 1;
       const W4Ahead<NT, GRAD ? 1 : W> cur = next;
       if (kb + WK < kb1) fetch(kb + WK, buf ^ 1, next);
-      const u32x4* xb = lds[buf] + (wm * MT * 32 + l32) * 16;
+      const u32x4* xb = lds + buf * BM * 16 + (wm * MT * 32 + l32) * 16;
       const int turn = (l32 & 15) ^ half;
       if (WK > 1 && kb >= kb1) {
         // the other waves' last block: nothing for this half
       } else if constexpr (!GRAD) {
         // What the zero points take away of two windows at a time -- of this block, or (one window to a block) of every
-        // second block and the one before it: lanes' halves hold a window each.
+        // second block and the one before it: the lanes' halves hold a window each.
+        const bool pair_now = W > 1 || buf || kb + WK >= kb1, there = W > 1 || buf || !half;
         float zx[PAIRS][MT], zz[PAIRS][NT];
-        const bool pair_now = W > 1 || (it & 1) || kb + WK >= kb1;
+        uint32_t zq[PAIRS][NT];
+        auto scaled_zeros = [&]() {
+#pragma unroll
+          for (int v = 0; v < PAIRS; ++v)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              zz[v][n] = there ? -(float)h_from_bits(zq[v][n]) * (float)h_from_bits(zq[v][n] >> 16) : 0.0f;  // exact: 11 x 11 bits
+        };
         if constexpr (XS) {
           if (pair_now) {
 #pragma unroll
             for (int v = 0; v < PAIRS; ++v) {
-              const bool there = W > 1 || (it & 1) || !half;
-              const int win = W > 1 ? kb * W + 2 * v + half : (it & 1) && !half ? kb - WK : kb;
+              const int win = W > 1 ? kb * W + 2 * v + half : buf && !half ? kb - WK : kb;
 #pragma unroll
               for (int m = 0; m < MT; ++m) {
                 const int r = (wm * MT + m) * 32 + l32;
                 zx[v][m] = p.xs[(int64_t)win * a.rows + row0 + (r < rows ? r : rows - 1)];
               }
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint32_t q = static_cast<const uint32_t*>(a.params)[pt[n] + w4_group(a, win * FS) * 16];
-                zz[v][n] = there ? -(float)h_from_bits(q) * (float)h_from_bits(q >> 16) : 0.0f;  // exact: 11 x 11 bits
-              }
+              for (int n = 0; n < NT; ++n) zq[v][n] = static_cast<const uint32_t*>(a.params)[pt[n] + w4_group(a, win * FS) * 16];
             }
+            // Two sets of waves, a compute unit's only tile, must not wait here for what they have just asked for (384 rows,
+            // 4096 x 14336: 84 us, 92 with this line for both); other tiles hide that and gain registers (2048 x 4096 x
+            // 4096: 88.5, 91 without).
+            if (WK == 1) scaled_zeros();
           }
         }
         f32x16 lo[MH][NT];
@@ -474,12 +488,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
         }
         if constexpr (XS) {
           if (pair_now) {
+            if (WK > 1) scaled_zeros();
 #pragma unroll
             for (int v = 0; v < PAIRS; ++v)
 #pragma unroll
-              for (int m = 0; m < MT; ++m)
+              for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(zx[v][m], zz[v][n], acc[m][n], 0, 0, 0);
+                for (int m = 0; m < MT; ++m) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(zx[v][m], zz[v][n], acc[m][n], 0, 0, 0);
           }
         }
       } else {
@@ -497,8 +512,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
           W4Scales<KIND> sc[SETS];
 #pragma unroll
           for (int g = 0; g < SETS; ++g) {
-            sc[g].s = lds_sc[buf][g][0][st * 2 + half];
-            if constexpr (SZ == 2) sc[g].z = lds_sc[buf][g][SZ - 1][st * 2 + half];
+            sc[g].s = lds_sc[(buf * SETS + g) * SZ * 16 + st * 2 + half];
+            if constexpr (SZ == 2) sc[g].z = lds_sc[((buf * SETS + g) * SZ + 1) * 16 + st * 2 + half];
           }
           u32x4 xv[MT];
 #pragma unroll
