@@ -257,9 +257,9 @@ template <int KIND> struct W4Scales {
 // weights, which are rounded once to float16 (W4Scales).  It runs in float16 for both types: rows of bfloat16 are brought
 // into its range by a power of two each (w4_half_row), where they lose nothing, while weights rounded to bfloat16 would add
 // as much error as the rounding of the result (2.4e-3 of the norm against 1.7e-3) and take more instructions to make.  The
-// scales along the contraction come with the block's rows through LDS, two to a lane (4096 x 4096 x 4096: 137 us, 149 with
-// loads between the products).  2048 rows through 4096 x 4096, one tile to a compute unit: 89 us with zero points, the matrix
-// cores busy in 0.33 of the cycles, the waves waiting for loads in 0.38; 4096 rows: 1.03 PFLOP/s, turning included.
+// scales along the contraction come with the block's rows through LDS, two to a lane (4096 x 4096 x 4096: 131 us, 149 with
+// loads between the products).  2048 rows through 4096 x 4096, one tile to a compute unit: 83 us with zero points, the matrix
+// cores busy in 0.35 of the cycles, the waves waiting for loads in 0.33; 4096 rows without: 1.05 PFLOP/s, turning included.
 template <int NT, int W> struct W4Ahead {  // what a wave holds of a block that is on its way
   u32x4 b[NT][2];
   uint32_t s[NT][W];
