@@ -107,8 +107,7 @@ class PackedWeight:
     def _describe(self):
         kind, values = _kind_of(self.wq_bits, self.datatype)
         L = _bind()
-        s = _W4(data=self.data.data_ptr() or None, params=self.params.data_ptr() or None, norm=self.norm.data_ptr() or None,
-                experts=self.experts or 1, n=self.n, k=self.k, group=max(self.group_size, 0), kind=kind)
+        s = _W4(experts=self.experts or 1, n=self.n, k=self.k, group=max(self.group_size, 0), kind=kind)
         if values is not None:
             s.values[:] = values
         for t, dtype, nbytes in ((self.data, torch.int32, L.mq_w4_data_bytes(self.experts or 1, self.n, self.k)),
@@ -119,11 +118,21 @@ class PackedWeight:
                 raise ValueError(f"not the tensors of a packed weight: {t.dtype} {tuple(t.shape)} on {t.device}")
         self._c = s
         self._ref = ctypes.byref(s)
+        self._at = None   # the addresses that _c holds
         self._need = {}   # workspace bytes by (dtype, rows, aligned, counted, grad)
-        self._device = self.data.device
+
+    def _taken(self):
+        """The description for a call, with the addresses that the tensors have now: `t.data = other` and their like keep
+        the tensor object and give its old memory back."""
+        at = (self.data.data_ptr(), self.params.data_ptr(), self.norm.data_ptr())
+        if at != self._at:
+            self._describe()
+            self._c.data, self._c.params, self._c.norm = at
+            self._at = at
+        return self._ref
 
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref", "_need", "_device")}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref", "_at", "_need")}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
@@ -131,7 +140,7 @@ class PackedWeight:
 
     @property
     def device(self):
-        return self._device
+        return self.data.device
 
     @property
     def shape(self):
@@ -147,7 +156,7 @@ class PackedWeight:
         """The float16 weight, with the bits that quant_int / quant_int_asym / quant_datatype return for it."""
         out = torch.empty(self.shape, dtype=torch.float16, device=self.device)
         with torch.cuda.device(self.device):
-            _lib.check(_bind().mq_w4_unpack(self._ref, out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+            _lib.check(_bind().mq_w4_unpack(self._taken(), out.data_ptr(), torch.cuda.current_stream().cuda_stream))
         return out
 
     def __repr__(self):
@@ -295,10 +304,11 @@ def _forward(x, weight, bias, counts, index):
     rows = x.shape[0]
     y = x.new_empty((rows, weight.n))
     if rows:
+        ref = weight._taken()
         x, ld = _rows_of(x)
         at = x.data_ptr()
         ws, wp, need = _workspace(weight, x, at, rows, ld, counts, 0)
-        rc = L.mq_linear4(weight._ref, at, _XDTYPES[x.dtype], rows, ld, None if bias is None else bias.data_ptr(),
+        rc = L.mq_linear4(ref, at, _XDTYPES[x.dtype], rows, ld, None if bias is None else bias.data_ptr(),
                           None if counts is None else counts.data_ptr(), y.data_ptr(), wp, need,
                           torch._C._cuda_getCurrentRawStream(index))
         if rc:
@@ -313,10 +323,11 @@ def _backward(dy, weight, counts, want_x, want_bias, index):
     db = dy.new_empty((n,) if weight.experts is None else (weight.experts, n)) if want_bias else None
     if not rows:
         return dx, None if db is None else db.zero_()
+    ref = weight._taken()
     dy, ld = _rows_of(dy)
     at = dy.data_ptr()
     ws, wp, need = _workspace(weight, dy, at, rows, ld, counts, want_x + 2 * want_bias)
-    rc = L.mq_linear4_grad(weight._ref, at, _XDTYPES[dy.dtype], rows, ld, None if counts is None else counts.data_ptr(),
+    rc = L.mq_linear4_grad(ref, at, _XDTYPES[dy.dtype], rows, ld, None if counts is None else counts.data_ptr(),
                            None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), wp, need,
                            torch._C._cuda_getCurrentRawStream(index))
     if rc:
@@ -349,7 +360,7 @@ def _check_operands(x, weight, bias):
         raise ValueError(f"float16 or bfloat16 activations are wanted, got {x.dtype}")
     if not x.dim() or x.shape[-1] != weight.k:
         raise ValueError(f"activations {tuple(x.shape)} do not fit a weight {tuple(weight.shape)}")
-    if x.device != weight._device:
+    if x.device != weight.data.device:
         raise ValueError(f"activations on {x.device}, weight on {weight.device}")
     if bias is not None:
         want = (weight.n,) if weight.experts is None else (weight.experts, weight.n)

@@ -1,0 +1,44 @@
+"""GPU: packed weights whose tensors are exchanged, moved, saved or changed under way; calls that are differentiated forwards
+or recorded."""
+import copy
+import io
+
+import pytest
+import torch
+import torch.nn as nn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def pk():
+    from quantization_amd import packed
+    return packed
+
+
+def layer(pk, seed=0, n=96, k=256, fmt="int4", bits=4, g=64, bias=True):
+    torch.manual_seed(seed)
+    return pk.PackedLinear(nn.Linear(k, n, bias=bias).half().cuda(), bits, fmt, g)
+
+
+def test_a_buffer_with_other_storage(pk):
+    """t.data = other: the next call reads the new storage, whatever happens to the old one."""
+    x = torch.randn(5, 256, device="cuda").half()
+    m = layer(pk)
+    want, deq = m(x), m.packed.dequantize()
+    for name in ("weight_data", "weight_params", "weight_norm"):
+        t = getattr(m, name)
+        old = t.detach()
+        t.data = t.data.clone()
+        old.fill_(-1)
+        assert torch.equal(m(x), want) and torch.equal(m.packed.dequantize(), deq), name
+    xg = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(m(xg), xg, torch.ones_like(want))
+    other = layer(pk)
+    assert torch.equal(dx, torch.autograd.grad(other(xg), xg, torch.ones_like(want))[0])
+    # away from the device under the same tensor object: refused, not read at the old address
+    for name in ("weight_data", "weight_params", "weight_norm"):
+        t = getattr(m, name)
+        t.data = t.data.cpu()
+    with pytest.raises(ValueError):
+        m(x)
