@@ -408,26 +408,50 @@ def packed_expert_linear(x, weight: PackedWeight, counts, bias=None):
     return _run(x, weight, bias, counts.contiguous())
 
 
+_BUFFERS = {"weight_data": "data", "weight_params": "params", "weight_norm": "norm"}   # of PackedLinear: its PackedWeight's
+
+
 class PackedLinear(nn.Module):
     """A Linear whose weight is held in 4 bits: quantizes src.weight with pack_weight; the bias stays a parameter."""
+
+    _packed = None   # the PackedWeight of the present buffers, once one has been asked for
 
     def __init__(self, src: nn.Linear, wq_bits: int = 4, datatype: str = "int4", group_size=None):
         super().__init__()
         self.in_features, self.out_features = src.in_features, src.out_features
-        self._packed = pack_weight(src.weight.data, wq_bits, datatype, group_size)
-        for name in ("data", "params", "norm"):
-            self.register_buffer("weight_" + name, getattr(self._packed, name))
-        self.bias = None if src.bias is None else nn.Parameter(src.bias.detach().to(self._packed.device),
+        p = pack_weight(src.weight.data, wq_bits, datatype, group_size)
+        self._form = (p.experts, p.n, p.k, p.group_size, p.wq_bits, p.datatype)
+        for name, of in _BUFFERS.items():
+            self.register_buffer(name, getattr(p, of))
+        self.bias = None if src.bias is None else nn.Parameter(src.bias.detach().to(p.device),
                                                                requires_grad=src.bias.requires_grad)
 
     @property
     def packed(self) -> PackedWeight:
         """The weight that the buffers hold (moved, loaded or assigned ones are taken up)."""
         p = self._packed
-        if p.data is not self.weight_data or p.params is not self.weight_params or p.norm is not self.weight_norm:
-            p = self._packed = PackedWeight(self.weight_data, self.weight_params, self.weight_norm, p.experts, p.n, p.k,
-                                            p.group_size, p.wq_bits, p.datatype)
+        if p is None or p.data is not self.weight_data or p.params is not self.weight_params or p.norm is not self.weight_norm:
+            p = self._packed = PackedWeight(self.weight_data, self.weight_params, self.weight_norm, *self._form)
         return p
+
+    # Wherever buffers are exchanged the PackedWeight goes with them: it would keep the old ones' memory.
+    def __setattr__(self, name, value):
+        super().__setattr__(name, value)
+        if name in _BUFFERS:
+            self._packed = None
+
+    def _apply(self, fn, recurse=True):
+        self._packed = None
+        return super()._apply(fn, recurse)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_packed"}
+
+    def __setstate__(self, state):
+        old = state.pop("_packed", None)   # modules saved before _form was kept
+        if old is not None:
+            state["_form"] = (old.experts, old.n, old.k, old.group_size, old.wq_bits, old.datatype)
+        super().__setstate__(state)
 
     def forward(self, x):
         return packed_linear(x, self.packed, self.bias)

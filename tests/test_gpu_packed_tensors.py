@@ -42,3 +42,21 @@ def test_a_buffer_with_other_storage(pk):
         t.data = t.data.cpu()
     with pytest.raises(ValueError):
         m(x)
+
+
+def test_a_layer_that_moves_away_frees_the_device(pk):
+    m = layer(pk, n=2048, k=2048, bias=False)
+    x = torch.randn(3, 2048, device="cuda").half()
+    want = m(x).clone()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    size = sum(b.numel() * b.element_size() for b in m.buffers())
+    m.cpu()
+    assert torch.cuda.memory_allocated() <= before - size
+    with pytest.raises(ValueError):
+        m(x)
+    assert torch.equal(m.cuda()(x), want)
+    back = io.BytesIO()
+    torch.save(m, back)
+    assert back.tell() < size + (1 << 16)
+    assert torch.equal(copy.deepcopy(m)(x), want)

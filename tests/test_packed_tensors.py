@@ -1,5 +1,9 @@
 """CPU: which tensors, addresses and formats a packed weight hands on, with a stand-in for the launches."""
+import copy
 import ctypes
+import io
+import pickle
+import weakref
 
 import pytest
 import torch
@@ -74,3 +78,50 @@ def test_a_tensor_with_other_storage_is_taken_up(launches):
     w.data.data = w.data.data[:-4].clone()
     with pytest.raises(ValueError):
         run(rows(), w)
+
+
+@pytest.fixture
+def host_linear(monkeypatch):
+    """PackedLinear on the host."""
+    monkeypatch.setattr(packed, "pack_weight",
+                        lambda w, bits, fmt, g: host_weight(w.shape[0], w.shape[1], g or 0, bits, fmt))
+    return lambda n=32, k=128, group=64, bits=4, fmt="int4": packed.PackedLinear(nn.Linear(k, n).half(), bits, fmt, group)
+
+
+BUFFERS = ("weight_data", "weight_params", "weight_norm")
+
+
+@pytest.mark.parametrize("way", ["applied", "assigned", "loaded"])
+def test_exchanged_buffers_are_let_go_at_once(host_linear, way):
+    """The weight that a module no longer holds takes no memory: moving it away frees the device's."""
+    m = host_linear()
+    assert m.packed.data is m.weight_data
+    old = [weakref.ref(getattr(m, b)) for b in BUFFERS]
+    if way == "applied":
+        m._apply(lambda t: t.clone())
+    elif way == "assigned":
+        for b in BUFFERS:
+            setattr(m, b, getattr(m, b).clone())
+    else:
+        m.load_state_dict({k: v.clone() for k, v in m.state_dict().items()}, assign=True)
+    assert [r() for r in old] == [None] * 3
+    assert m.packed.data is m.weight_data and m.packed.params is m.weight_params and m.packed.norm is m.weight_norm
+
+
+def test_a_saved_module_holds_its_weight_once(host_linear):
+    m = host_linear(256, 1024)
+    m.packed
+    once = sum(getattr(m, b).numel() * getattr(m, b).element_size() for b in BUFFERS)
+    for again in (pickle.loads(pickle.dumps(m)), copy.deepcopy(m)):
+        assert again.packed.data is again.weight_data and again.packed.shape == m.packed.shape
+        assert repr(again) == repr(m)
+    m._buffers["weight_data"] = m.weight_data.clone()   # past the module's own ways
+    file = io.BytesIO()
+    torch.save(m, file)
+    assert once < file.tell() < once + (1 << 16)
+    assert m.packed.data is m.weight_data
+    state = dict(m.__dict__, _packed=m.packed)          # as modules were saved that kept no description of their own
+    del state["_form"]
+    old = packed.PackedLinear.__new__(packed.PackedLinear)
+    old.__setstate__(state)
+    assert repr(old) == repr(m)
