@@ -131,6 +131,10 @@ class PackedWeight:
             self._at = at
         return self._ref
 
+    def _versions(self):
+        """How often each tensor has been written in place (tensors of inference mode do not say)."""
+        return [0 if t.is_inference() else t._version for t in (self.data, self.params, self.norm)]
+
     def __getstate__(self):
         return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref", "_at", "_need")}
 
@@ -338,7 +342,8 @@ def _backward(dy, weight, counts, want_x, want_bias, index):
 class _PackedProduct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, weight, counts):
-        ctx.weight = weight
+        # (the weight's tensors are not saved: hooks that move what is saved would carry the whole weight to and fro)
+        ctx.weight, ctx.versions = weight, weight._versions()
         ctx.save_for_backward(counts)
         return _on_device(_forward, x, weight, bias, counts)
 
@@ -347,6 +352,9 @@ class _PackedProduct(torch.autograd.Function):
     def backward(ctx, dy):
         counts, = ctx.saved_tensors
         want_x, want_bias = ctx.needs_input_grad[:2]
+        if want_x and ctx.weight._versions() != ctx.versions:
+            raise RuntimeError("the packed weight has been written in place since the forward pass: its gradient would be "
+                               "that of another weight")
         dx, db = _on_device(_backward, dy, ctx.weight, counts, want_x, want_bias)
         return dx, db, None, None
 

@@ -60,3 +60,19 @@ def test_a_layer_that_moves_away_frees_the_device(pk):
     torch.save(m, back)
     assert back.tell() < size + (1 << 16)
     assert torch.equal(copy.deepcopy(m)(x), want)
+
+
+def test_a_state_dict_loaded_between_forward_and_backward(pk):
+    m, other = layer(pk), layer(pk, seed=1)
+    x = torch.randn(40, 256, device="cuda").half().requires_grad_()
+    dy = torch.randn(40, 96, device="cuda").half()
+    want, = torch.autograd.grad(m(x), x, dy)
+    y = m(x)
+    m.load_state_dict(other.state_dict(), assign=True)     # beside the forward's weight
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+    m = layer(pk)
+    y = m(x)
+    m.load_state_dict({k: v.clone() for k, v in other.state_dict().items()})
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, x, dy)
+    assert torch.equal(m(x), other(x))

@@ -125,3 +125,39 @@ def test_a_saved_module_holds_its_weight_once(host_linear):
     old = packed.PackedLinear.__new__(packed.PackedLinear)
     old.__setstate__(state)
     assert repr(old) == repr(m)
+
+
+def test_a_weight_changed_between_forward_and_backward(launches, host_linear):
+    """As torch does for the weights of its own products: the gradient is that of the forward's weight, or an error."""
+    def forward(w):
+        x = rows().requires_grad_()
+        b = torch.zeros(w.n, dtype=torch.float16, requires_grad=True)
+        return x, b, packed._PackedProduct.apply(x, b, w, None)
+
+    for name in ("data", "params", "norm"):
+        w = host_weight()
+        x, b, y = forward(w)
+        getattr(w, name).add_(1)
+        with pytest.raises(RuntimeError, match="forward"):
+            torch.autograd.grad(y, x, torch.ones_like(y))
+        x, b, y = forward(w)                        # the bias's gradient does not read the weight
+        getattr(w, name).add_(1)
+        torch.autograd.grad(y, b, torch.ones_like(y))
+        x, b, y = forward(w)
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    # a state dict loaded under way: copied into the buffers, or (assign) beside the forward's
+    m = host_linear()
+    state = {k: v.clone() for k, v in m.state_dict().items()}
+    x, b, y = forward(m.packed)
+    m.load_state_dict(state)
+    with pytest.raises(RuntimeError, match="forward"):
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    x, b, y = forward(m.packed)
+    was = addresses(m.packed)
+    m.load_state_dict(state, assign=True)
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    assert launches.seen[-1] == was != addresses(m.packed)
+    with torch.inference_mode():                    # tensors without versions
+        w = host_weight()
+    x, b, y = forward(w)
+    torch.autograd.grad(y, x, torch.ones_like(y))
