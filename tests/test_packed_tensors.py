@@ -140,9 +140,10 @@ def test_a_weight_changed_between_forward_and_backward(launches, host_linear):
         getattr(w, name).add_(1)
         with pytest.raises(RuntimeError, match="forward"):
             torch.autograd.grad(y, x, torch.ones_like(y))
-        x, b, y = forward(w)                        # the bias's gradient does not read the weight
+        b = torch.zeros(w.n, dtype=torch.float16, requires_grad=True)
+        y = packed._PackedProduct.apply(rows(), b, w, None)
         getattr(w, name).add_(1)
-        torch.autograd.grad(y, b, torch.ones_like(y))
+        torch.autograd.grad(y, b, torch.ones_like(y))      # a bias's gradient alone does not read the weight
         x, b, y = forward(w)
         torch.autograd.grad(y, x, torch.ones_like(y))
     # a state dict loaded under way: copied into the buffers, or (assign) beside the forward's
