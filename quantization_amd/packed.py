@@ -15,6 +15,7 @@ import ctypes
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -345,6 +346,7 @@ class _PackedProduct(torch.autograd.Function):
         # (the weight's tensors are not saved: hooks that move what is saved would carry the whole weight to and fro)
         ctx.weight, ctx.versions = weight, weight._versions()
         ctx.save_for_backward(counts)
+        ctx.save_for_forward(counts)
         return _on_device(_forward, x, weight, bias, counts)
 
     @staticmethod
@@ -357,6 +359,14 @@ class _PackedProduct(torch.autograd.Function):
                                "that of another weight")
         dx, db = _on_device(_backward, dy, ctx.weight, counts, want_x, want_bias)
         return dx, db, None, None
+
+    @staticmethod
+    def jvp(ctx, dx, dbias, *_):
+        """Linear in x and the bias: the tangent is the product of the tangents."""
+        counts, = ctx.saved_tensors
+        if dx._is_zerotensor():   # (one without memory)
+            dx = torch.zeros(dx.shape, dtype=dx.dtype, device=dx.device)
+        return _run(dx, ctx.weight, dbias, counts)
 
 
 def _check_operands(x, weight, bias):
@@ -380,7 +390,7 @@ def _check_operands(x, weight, bias):
 
 
 def _run(x, weight, bias, counts):
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
         return _PackedProduct.apply(x, bias, weight, counts)
     return _on_device(_forward, x, weight, bias, counts)
 

@@ -6,6 +6,7 @@ import io
 import pytest
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as fa
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +77,28 @@ def test_a_state_dict_loaded_between_forward_and_backward(pk):
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y, x, dy)
     assert torch.equal(m(x), other(x))
+
+
+def test_forward_mode_differentiation(pk):
+    """The tangent of a product is the product of the tangents, whether or not gradients are wanted too."""
+    w = layer(pk, fmt="int4_asym").packed
+    x, t = (torch.randn(5, 256, device="cuda").half() for _ in range(2))
+    b, bt = (torch.randn(96, device="cuda").half() for _ in range(2))
+    for grad in (False, True):
+        with fa.dual_level(), torch.set_grad_enabled(grad):
+            y, yt = fa.unpack_dual(pk.packed_linear(fa.make_dual(x, t), w, fa.make_dual(b, bt)))
+            assert torch.equal(y, pk.packed_linear(x, w, b)) and torch.equal(yt, pk.packed_linear(t, w, bt))
+            y, yt = fa.unpack_dual(pk.packed_linear(fa.make_dual(x, t), w, b))
+            assert torch.equal(yt, pk.packed_linear(t, w))
+            _, yt = fa.unpack_dual(pk.packed_linear(x, w, fa.make_dual(b, bt)))
+            assert torch.equal(yt, bt.expand(5, 96))
+            assert fa.unpack_dual(pk.packed_linear(x, w, b)).tangent is None
+    e = pk.pack_weight(torch.randn(3, 96, 256, device="cuda").half(), 4, "int4", 64)
+    c, be, bet = torch.tensor([2, 0, 2], device="cuda"), torch.randn(3, 96, device="cuda").half(), torch.randn(3, 96, device="cuda").half()
+    with fa.dual_level():
+        y, yt = fa.unpack_dual(pk.packed_expert_linear(fa.make_dual(x, t), e, c, fa.make_dual(be, bet)))
+    assert torch.equal(y, pk.packed_expert_linear(x, e, c, be)) and torch.equal(yt, pk.packed_expert_linear(t, e, c, bet))
+    with pytest.raises(RuntimeError):      # transforms that wrap tensors
+        torch.func.jvp(lambda v: pk.packed_linear(v, w), (x,), (t,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: pk.packed_linear(v, w))(x[:, None])

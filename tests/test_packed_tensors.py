@@ -8,29 +8,31 @@ import weakref
 import pytest
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as fa
 
 from quantization_amd import packed
 
 
 class StandIn:
-    """libmq.so with launches that only note the weight's addresses; sizes come from the library itself."""
+    """libmq.so with launches that only note the addresses of the weight and the rows; sizes come from the library itself."""
 
     def __init__(self, real):
-        self.real, self.seen = real, []
+        self.real, self.seen, self.rows = real, [], []
 
     def __getattr__(self, name):
         return getattr(self.real, name)
 
-    def _note(self, ref):
+    def _note(self, ref, x):
+        self.rows.append(x)
         c = ctypes.cast(ref, ctypes.POINTER(packed._W4)).contents
         self.seen.append((c.data, c.params, c.norm))
         return 0
 
-    def mq_linear4(self, ref, *args):
-        return self._note(ref)
+    def mq_linear4(self, ref, x, *args):
+        return self._note(ref, x)
 
-    def mq_linear4_grad(self, ref, *args):
-        return self._note(ref)
+    def mq_linear4_grad(self, ref, dy, *args):
+        return self._note(ref, dy)
 
 
 @pytest.fixture
@@ -162,3 +164,25 @@ def test_a_weight_changed_between_forward_and_backward(launches, host_linear):
         w = host_weight()
     x, b, y = forward(w)
     torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_differentiation_has_a_tangent(launches, grad):
+    """The product is linear in x and in the bias: the tangent is one more product."""
+    w = host_weight()
+    bias = torch.zeros(w.n, dtype=torch.float16)
+    for with_x, with_bias in ((True, True), (True, False), (False, True)):
+        with fa.dual_level(), torch.set_grad_enabled(grad):
+            x = fa.make_dual(rows(), rows()) if with_x else rows()
+            b = fa.make_dual(bias, torch.ones_like(bias)) if with_bias else bias
+            before = len(launches.seen)
+            y = packed._run(x, w, b, None)
+            assert fa.unpack_dual(y).tangent is not None
+            assert fa.unpack_dual(y).tangent.shape == y.shape
+            assert len(launches.seen) == before + 2
+    with fa.dual_level():     # a tangent without memory
+        y = packed._run(fa.make_dual(rows(), torch._efficientzerotensor((3, 128), dtype=torch.float16)), w, None, None)
+        assert fa.unpack_dual(y).tangent is not None and launches.rows[-1]
+    with fa.dual_level():     # nothing to differentiate
+        y = packed._run(rows(), w, bias, None)
+        assert fa.unpack_dual(y).tangent is None
