@@ -12,11 +12,13 @@ Activations are float16 or bfloat16, sums float32, results rounded once.  The re
 (_LinearDump, quant_weight.py:876-914) and multiplies by the dequantized float16 weight; there is no CPU compute path.
 """
 import ctypes
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 from .fused import TABLE_LISTS, lut_values, require_device
@@ -156,17 +158,28 @@ class PackedWeight:
         return PackedWeight(self.data.to(device), self.params.to(device), self.norm.to(device), self.experts, self.n, self.k,
                             self.group_size, self.wq_bits, self.datatype)
 
+    def _operands(self):
+        """The weight as the registered operators take it."""
+        return (self.data, self.params, self.norm), (self.experts or 0, self.n, self.k, self.group_size, self.wq_bits, self.datatype)
+
     @torch.no_grad()
     def dequantize(self):
         """The float16 weight, with the bits that quant_int / quant_int_asym / quant_datatype return for it."""
-        out = torch.empty(self.shape, dtype=torch.float16, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_bind().mq_w4_unpack(self._taken(), out.data_ptr(), torch.cuda.current_stream().cuda_stream))
-        return out
+        if _recorded(self.data):
+            tensors, form = self._operands()
+            return torch.ops.quantization_amd.packed_dequantize(*tensors, *form)
+        return _dequantize(self)
 
     def __repr__(self):
         g = {0: "per row", -1: "per tensor"}.get(self.group_size, f"groups of {self.group_size}")
         return f"PackedWeight({tuple(self.shape)}, {self.wq_bits}-bit {self.datatype}, {g}, {self.device})"
+
+
+def _dequantize(weight):
+    out = torch.empty(weight.shape, dtype=torch.float16, device=weight.device)
+    with torch.cuda.device(weight.device):
+        _lib.check(_bind().mq_w4_unpack(weight._taken(), out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    return out
 
 
 @torch.no_grad()
@@ -176,6 +189,8 @@ def pack_codes(q, scale, zp=None, wq_bits: int = 4, datatype: str = "int4", grou
     q: int8 / uint8 codes (integers) or float16 table values, [N, K] or [N, G, group_size]; scale (and, for asymmetric
     integers, zp): float16, [N, G] per group, [N] per row, [] per tensor.  With a leading dimension E on all of them: a
     stack of experts.  Groups are multiples of 32 that divide K; rows may have any length."""
+    if _compiling() or _tracing() or get_proxy_mode() is not None:
+        raise RuntimeError("packing a weight cannot be recorded: pack it beforehand")
     kind, values = _kind_of(wq_bits, datatype)
     g = _group(group_size)
     experts = scale.dim() - (2 if g > 0 else 0 if g == -1 else 1)
@@ -340,6 +355,95 @@ def _backward(dy, weight, counts, want_x, want_bias, index):
     return dx, db
 
 
+# ---- where someone records or interprets torch's operators -------------------------------------------------
+# The calls above hand addresses to the library, which nothing in torch sees: a recorder would keep the allocation of the
+# result alone and replay that.  So wherever one is at work the same calls run as operators of torch's own.
+_PLAIN = {torch.Tensor, nn.Parameter, type(None)}
+_compiling, _tracing, _modes = torch.compiler.is_compiling, torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+
+
+def _recorded(x, bias=None, counts=None):
+    """True under torch.compile, torch.jit.trace, a dispatch mode (make_fx, torch.export, fake tensors) or for tensors of
+    another class."""
+    return (_compiling() or _tracing() or _modes() > 0 or type(x) not in _PLAIN or type(bias) not in _PLAIN
+            or type(counts) not in _PLAIN)
+
+
+@torch.library.custom_op("quantization_amd::packed_product", mutates_args=(), device_types="cuda")
+def _product_op(x: torch.Tensor, data: torch.Tensor, params: torch.Tensor, norm: torch.Tensor, bias: Optional[torch.Tensor],
+                counts: Optional[torch.Tensor], experts: int, n: int, k: int, group_size: int, wq_bits: int,
+                datatype: str) -> torch.Tensor:
+    weight = PackedWeight(data, params, norm, experts or None, n, k, group_size, wq_bits, datatype)
+    bias, counts = _check_operands(x, weight, bias), _check_rows(x, weight, counts)
+    return _on_device(_forward, x, weight, bias, counts)
+
+
+@_product_op.register_fake
+def _(x, data, params, norm, bias, counts, experts, n, k, group_size, wq_bits, datatype):
+    return x.new_empty((x.shape[0], n))
+
+
+@torch.library.custom_op("quantization_amd::packed_product_grad", mutates_args=(), device_types="cuda")
+def _gradient_op(dy: torch.Tensor, data: torch.Tensor, params: torch.Tensor, norm: torch.Tensor,
+                 counts: Optional[torch.Tensor], experts: int, n: int, k: int, group_size: int, wq_bits: int, datatype: str,
+                 want_x: bool, want_bias: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What is not wanted comes back empty."""
+    weight = PackedWeight(data, params, norm, experts or None, n, k, group_size, wq_bits, datatype)
+    if dy.dtype not in _XDTYPES or dy.dim() != 2 or dy.shape[1] != n or dy.device != data.device:
+        raise ValueError(f"a gradient {dy.dtype} {tuple(dy.shape)} on {dy.device} does not fit a weight {tuple(weight.shape)}")
+    dx, db = None, None
+    if want_x or want_bias:
+        dx, db = _on_device(_backward, dy, weight, _check_rows(dy, weight, counts), want_x, want_bias)
+    return dy.new_empty(0) if dx is None else dx, dy.new_empty(0) if db is None else db
+
+
+@_gradient_op.register_fake
+def _(dy, data, params, norm, counts, experts, n, k, group_size, wq_bits, datatype, want_x, want_bias):
+    db = ((experts, n) if experts else (n,)) if want_bias else (0,)
+    return dy.new_empty((dy.shape[0], k) if want_x else (0,)), dy.new_empty(db)
+
+
+def _product_op_setup(ctx, inputs, output):
+    x, data, params, norm, bias, counts, *form = inputs
+    ctx.save_for_backward(data, params, norm, counts)
+    ctx.form = form
+
+
+def _product_op_backward(ctx, dy):
+    want_x, want_bias = ctx.needs_input_grad[0], ctx.needs_input_grad[4]
+    dx, db = torch.ops.quantization_amd.packed_product_grad(dy, *ctx.saved_tensors, *ctx.form, want_x, want_bias)
+    return (dx if want_x else None, None, None, None, db if want_bias else None) + (None,) * 7
+
+
+_product_op.register_autograd(_product_op_backward, setup_context=_product_op_setup)
+
+
+@torch.library.custom_op("quantization_amd::packed_dequantize", mutates_args=(), device_types="cuda")
+def _dequantize_op(data: torch.Tensor, params: torch.Tensor, norm: torch.Tensor, experts: int, n: int, k: int,
+                   group_size: int, wq_bits: int, datatype: str) -> torch.Tensor:
+    return _dequantize(PackedWeight(data, params, norm, experts or None, n, k, group_size, wq_bits, datatype))
+
+
+@_dequantize_op.register_fake
+def _(data, params, norm, experts, n, k, group_size, wq_bits, datatype):
+    return data.new_empty((experts, n, k) if experts else (n, k), dtype=torch.float16)
+
+
+def _product(x, weight, bias, counts):
+    if _recorded(x, bias, counts):
+        tensors, form = weight._operands()
+        return torch.ops.quantization_amd.packed_product(x, *tensors, bias, counts, *form)
+    return _on_device(_forward, x, weight, bias, counts)
+
+
+def _gradient(dy, weight, counts, want_x, want_bias):
+    if _recorded(dy, None, counts):
+        tensors, form = weight._operands()
+        dx, db = torch.ops.quantization_amd.packed_product_grad(dy, *tensors, counts, *form, want_x, want_bias)
+        return dx if want_x else None, db if want_bias else None
+    return _on_device(_backward, dy, weight, counts, want_x, want_bias)
+
+
 class _PackedProduct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, weight, counts):
@@ -347,7 +451,7 @@ class _PackedProduct(torch.autograd.Function):
         ctx.weight, ctx.versions = weight, weight._versions()
         ctx.save_for_backward(counts)
         ctx.save_for_forward(counts)
-        return _on_device(_forward, x, weight, bias, counts)
+        return _product(x, weight, bias, counts)
 
     @staticmethod
     @once_differentiable
@@ -357,7 +461,7 @@ class _PackedProduct(torch.autograd.Function):
         if want_x and ctx.weight._versions() != ctx.versions:
             raise RuntimeError("the packed weight has been written in place since the forward pass: its gradient would be "
                                "that of another weight")
-        dx, db = _on_device(_backward, dy, ctx.weight, counts, want_x, want_bias)
+        dx, db = _gradient(dy, ctx.weight, counts, want_x, want_bias)
         return dx, db, None, None
 
     @staticmethod
@@ -389,8 +493,25 @@ def _check_operands(x, weight, bias):
     return bias
 
 
+def _check_rows(x, weight, counts):
+    """The counts of experts' rows as the library reads them; None for a single weight."""
+    if weight.experts is None:
+        if counts is not None:
+            raise ValueError("counts go with a stack of experts")
+        return None
+    if not isinstance(counts, torch.Tensor) or counts.dtype not in (torch.int32, torch.int64) \
+            or tuple(counts.shape) != (weight.experts,) or counts.device != x.device:
+        raise ValueError(f"counts: int32 or int64 [{weight.experts}] on {x.device} wanted")
+    if counts.dtype == torch.int64:
+        counts = counts.clamp(0, x.shape[0]).to(torch.int32)
+    return counts.contiguous()
+
+
 def _run(x, weight, bias, counts):
-    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
+    forwards = forward_ad._current_level >= 0
+    if not forwards and _recorded(x, bias, counts):
+        return _product(x, weight, bias, counts)   # (the operator knows its gradient)
+    if forwards or torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
         return _PackedProduct.apply(x, bias, weight, counts)
     return _on_device(_forward, x, weight, bias, counts)
 
@@ -418,12 +539,7 @@ def packed_expert_linear(x, weight: PackedWeight, counts, bias=None):
         raise ValueError("a single weight goes through packed_linear")
     if x.dim() != 2:
         raise ValueError(f"rows [R, {weight.k}] are wanted, got {tuple(x.shape)}")
-    if not isinstance(counts, torch.Tensor) or counts.dtype not in (torch.int32, torch.int64) \
-            or tuple(counts.shape) != (weight.experts,) or counts.device != x.device:
-        raise ValueError(f"counts: int32 or int64 [{weight.experts}] on {x.device} wanted")
-    if counts.dtype == torch.int64:
-        counts = counts.clamp(0, x.shape[0]).to(torch.int32)
-    return _run(x, weight, bias, counts.contiguous())
+    return _run(x, weight, bias, _check_rows(x, weight, counts))
 
 
 _BUFFERS = {"weight_data": "data", "weight_params": "params", "weight_norm": "norm"}   # of PackedLinear: its PackedWeight's

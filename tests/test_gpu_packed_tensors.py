@@ -6,7 +6,10 @@ import io
 import pytest
 import torch
 import torch.nn as nn
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad as fa
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +105,89 @@ def test_forward_mode_differentiation(pk):
         torch.func.jvp(lambda v: pk.packed_linear(v, w), (x,), (t,))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda v: pk.packed_linear(v, w))(x[:, None])
+
+
+class Counting(TorchDispatchMode):
+    """Notes the operators that run inside."""
+
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(func.__name__)
+        return func(*args, **(kwargs or {}))
+
+
+class Named(torch.Tensor):
+    pass
+
+
+def test_recorded_products_replay_what_was_recorded(pk):
+    """Traced, captured, exported and compiled programs multiply; they do not return memory that nobody has written."""
+    m = layer(pk, fmt="int4_asym")
+    stack = pk.pack_weight(torch.randn(3, 96, 256, device="cuda").half(), 4, "fp4", 64)
+    counts = torch.tensor([2, 1, 2], device="cuda")
+    x, x2 = (torch.randn(5, 256, device="cuda").half() for _ in range(2))
+    w, b = m.packed, m.bias.detach()
+    both = lambda x: (pk.packed_linear(x, w, b), pk.packed_expert_linear(x, stack, counts), stack.dequantize())
+    with torch.no_grad():
+        want = [t.clone() for t in both(x2)]
+        traced = torch.jit.trace(both, x)
+        file = io.BytesIO()
+        layer_traced = torch.jit.trace(m, x)
+        torch.jit.save(layer_traced, file)
+        file.seek(0)
+        programs = {"traced": traced, "make_fx": make_fx(both)(x),
+                    "compiled": torch.compile(both, backend="aot_eager", fullgraph=True)}
+        for name, f in programs.items():
+            torch.full((1 << 16,), float("nan"), device="cuda")       # (what the allocator hands out next)
+            assert all(torch.equal(a, b) for a, b in zip(f(x2), want)), name
+        for f in (layer_traced, torch.jit.load(file), torch.export.export(m, (x,), strict=False).module()):
+            assert torch.equal(f(x2), want[0])
+    # with gradients: each program's own backward pass
+    xg = x2.clone().requires_grad_()
+    dy = torch.randn(5, 96, device="cuda").half()
+    want = torch.autograd.grad(m(xg), (xg, m.bias), dy)
+    for f in (torch.jit.trace(m, x), torch.compile(m, backend="aot_eager", fullgraph=True)):
+        y = f(xg)
+        assert torch.equal(y, m(xg))
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (xg, m.bias), dy), want))
+
+    def gradients(x, dy):
+        x = x.detach().requires_grad_()
+        return torch.autograd.grad(pk.packed_linear(x, m.packed), x, dy)[0]
+
+    assert torch.equal(make_fx(gradients)(x, dy)(x2, dy), want[0])
+    # others that look on: the operator has a name, the results are the same
+    with Counting() as seen:
+        y = m(xg)
+        got = torch.autograd.grad(y, (xg, m.bias), dy)
+    assert "packed_product.default" in seen.names and "packed_product_grad.default" in seen.names
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y = m(xg)
+    with Counting() as seen:                                          # the backward pass alone
+        got = torch.autograd.grad(y, (xg, m.bias), dy)
+    assert "packed_product_grad.default" in seen.names and all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        assert torch.equal(torch.Tensor(m(x2.as_subclass(Named))), m(x2))
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        assert m(mode.from_tensor(x)).shape == (5, 96)
+    assert torch.equal(m(xg), y)
+
+
+def test_the_operators_refuse_what_does_not_fit(pk):
+    w = layer(pk).packed
+    tensors, form = w._operands()
+    x, dy = torch.zeros(3, 256, device="cuda").half(), torch.zeros(3, 96, device="cuda").half()
+    f, g = torch.ops.quantization_amd.packed_product, torch.ops.quantization_amd.packed_product_grad
+    c = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for bad in (lambda: f(x[:, :255], *tensors, None, None, *form), lambda: f(x[0], *tensors, None, None, *form),
+                lambda: f(x, *tensors, dy[0, :95], None, *form), lambda: f(x, *tensors, None, c, *form),
+                lambda: f(x, *tensors, None, None, 2, *form[1:]), lambda: f(x, tensors[0][:4], *tensors[1:], None, None, *form),
+                lambda: g(x, *tensors, None, *form, True, True), lambda: g(dy.float(), *tensors, None, *form, True, True),
+                lambda: g(dy, *tensors, c, *form, True, True)):
+        with pytest.raises(ValueError):
+            bad()
+    dx, db = g(dy, *tensors, None, *form, False, False)
+    assert not dx.numel() and not db.numel()

@@ -8,7 +8,9 @@ import weakref
 import pytest
 import torch
 import torch.nn as nn
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad as fa
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from quantization_amd import packed
 
@@ -186,3 +188,48 @@ def test_forward_mode_differentiation_has_a_tangent(launches, grad):
     with fa.dual_level():     # nothing to differentiate
         y = packed._run(rows(), w, bias, None)
         assert fa.unpack_dual(y).tangent is None
+
+
+def fakes(mode, w):
+    with mode:
+        at = lambda t: torch.empty(t.shape, dtype=t.dtype, device="cuda")
+        return packed.PackedWeight(at(w.data), at(w.params), at(w.norm), w.experts, w.n, w.k, w.group_size, w.wq_bits, w.datatype)
+
+
+def test_a_recorded_product_is_an_operator_of_the_graph():
+    """Not the allocation of its result alone, which a replay would return unwritten."""
+    mode = FakeTensorMode()
+    w = fakes(mode, host_weight())
+    with mode:
+        x, b = (torch.empty(s, dtype=torch.float16, device="cuda") for s in ((4, 3, 128), (32,)))
+        c = torch.empty(1, dtype=torch.int64, device="cuda")
+    e = packed.PackedWeight(w.data, w.params, w.norm, 1, w.n, w.k, w.group_size, w.wq_bits, w.datatype)
+    names = lambda g: [n.target.__name__ for n in g.graph.nodes if n.op == "call_function"]
+    g = make_fx(lambda x, b: packed.packed_linear(x, w, b))(x, b)
+    assert "packed_product.default" in names(g)
+    g = make_fx(lambda x, c, b: packed.packed_expert_linear(x, e, c, b))(x[0], c, b[None])
+    assert "packed_product.default" in names(g)
+    assert "packed_dequantize.default" in names(make_fx(lambda x: w.dequantize() + x)(x[0, 0]))
+    with mode:      # shapes and types alone
+        assert packed.packed_linear(x, w, b).shape == (4, 3, 32) and w.dequantize().shape == (32, 128)
+        tensors, form = w._operands()
+        dx, db = torch.ops.quantization_amd.packed_product_grad(x[0, :, :32], *tensors, None, *form, True, False)
+        assert dx.shape == (3, 128) and db.shape == (0,) and dx.dtype == torch.float16
+
+
+def test_what_cannot_be_recorded_raises(launches):
+    w = host_weight()
+    with pytest.raises(NotImplementedError):        # (the operator has no host form)
+        torch.jit.trace(lambda x: packed._run(x, w, None, None), rows())
+    with pytest.raises(NotImplementedError):
+        make_fx(lambda x: packed._run(x, w, None, None))(rows())
+    assert not launches.seen
+    q, s = torch.zeros(32, 128, dtype=torch.int8), torch.ones(32, 2, dtype=torch.float16)
+    for record in (torch.jit.trace, lambda f, a: make_fx(f)(*a)):
+        with pytest.raises(RuntimeError, match="recorded"):
+            record(lambda q, s: packed.pack_codes(q, s, group_size=64).data, (q, s))
+    x, b = rows(), torch.zeros(32, dtype=torch.float16)
+    for f in (lambda: torch.ops.quantization_amd.packed_product(x, w.data, w.params, w.norm, b, None, 0, 32, 128, 64, 4, "int4"),
+              lambda: torch.ops.quantization_amd.packed_dequantize(w.data, w.params, w.norm, 0, 32, 128, 64, 4, "int4")):
+        with pytest.raises(NotImplementedError):
+            f()
