@@ -12,6 +12,7 @@ Activations are float16 or bfloat16, sums float32, results rounded once.  The re
 (_LinearDump, quant_weight.py:876-914) and multiplies by the dequantized float16 weight; there is no CPU compute path.
 """
 import ctypes
+import warnings
 from typing import Optional, Tuple
 
 import torch
@@ -586,6 +587,33 @@ class PackedLinear(nn.Module):
         if old is not None:
             state["_form"] = (old.experts, old.n, old.k, old.group_size, old.wq_bits, old.datatype)
         super().__setstate__(state)
+
+    # A state dict says what its codes mean: the buffers of two formats may have the same sizes.
+    def _format(self):
+        _, n, k, group, bits, datatype = self._form
+        kind, values = _kind_of(bits, datatype)
+        name = {INT_ASYM: "asymmetric integers", INT_SYM: "symmetric integers", FP4: "fp4"}.get(kind) or \
+            "table " + " ".join(f"{v:g}" for v in values)
+        rows = group <= 0 or group == k and k % 128 == 0    # (one group: the same parameters)
+        return f"{n} x {k}, {name}, {'one scale per row' if rows else f'groups of {group}'}"
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "weight_format"] = torch.tensor(list(self._format().encode()), dtype=torch.uint8)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        key = prefix + "weight_format"
+        if key in state_dict:
+            theirs = bytes(state_dict[key].tolist()).decode(errors="replace")
+            if theirs != self._format():   # nothing of it is taken over
+                error_msgs.append(f"{key}: the format of the state dict's weight is \"{theirs}\", this module's "
+                                  f"\"{self._format()}\"")
+                return
+        elif prefix + "weight_data" in state_dict:
+            warnings.warn(f"{key} is missing: a weight of another format would be decoded wrongly", stacklevel=2)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if key in unexpected_keys:
+            unexpected_keys.remove(key)
 
     def forward(self, x):
         return packed_linear(x, self.packed, self.bias)

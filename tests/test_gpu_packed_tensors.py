@@ -191,3 +191,16 @@ def test_the_operators_refuse_what_does_not_fit(pk):
             bad()
     dx, db = g(dy, *tensors, None, *form, False, False)
     assert not dx.numel() and not db.numel()
+
+
+def test_a_state_dict_of_another_format_is_refused(pk):
+    x = torch.randn(5, 256, device="cuda").half()
+    m, other = layer(pk), layer(pk, fmt="fp4")
+    want = m(x)
+    for assign in (False, True):
+        with pytest.raises(RuntimeError):
+            m.load_state_dict(other.state_dict(), assign=assign)
+        assert torch.equal(m(x), want)
+    again = layer(pk, seed=1)
+    again.load_state_dict({k: v.cpu() for k, v in m.state_dict().items()})
+    assert torch.equal(again(x), want)

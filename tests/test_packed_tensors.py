@@ -48,7 +48,7 @@ def launches(monkeypatch):
 
 def host_weight(n=32, k=128, group=64, bits=4, fmt="int4", fill=0):
     """A weight whose tensors lie on the host."""
-    c = packed._W4(experts=1, n=n, k=k, group=group, kind=packed._kind_of(bits, fmt)[0])
+    c = packed._W4(experts=1, n=n, k=k, group=max(group, 0), kind=packed._kind_of(bits, fmt)[0])
     L = packed._bind()
     data = torch.full((L.mq_w4_data_bytes(1, n, k) // 4,), fill, dtype=torch.int32)
     params = torch.full((L.mq_w4_params_bytes(ctypes.byref(c)) // 2,), fill, dtype=torch.int16)
@@ -233,3 +233,42 @@ def test_what_cannot_be_recorded_raises(launches):
               lambda: torch.ops.quantization_amd.packed_dequantize(w.data, w.params, w.norm, 0, 32, 128, 64, 4, "int4")):
         with pytest.raises(NotImplementedError):
             f()
+
+
+def test_a_state_dict_says_its_format(host_linear):
+    """int4 and fp4 have buffers of the same sizes: the one's codes are not the other's."""
+    forms = [dict(), dict(fmt="fp4"), dict(fmt="flint4"), dict(fmt="fp4_er_pos"), dict(fmt="fp3", bits=3)]
+    for a in forms:
+        state = host_linear(**a).state_dict()
+        for b in forms:
+            m = host_linear(**b)
+            for assign in (False, True):
+                for strict in (False, True):
+                    if a == b:
+                        m.load_state_dict(state, strict=strict, assign=assign)
+                        continue
+                    kept = {k: v.clone() for k, v in m.state_dict().items()}
+                    state["weight_data"].fill_(7)
+                    with pytest.raises(RuntimeError, match="format"):
+                        m.load_state_dict(state, strict=strict, assign=assign)
+                    assert all(torch.equal(v, kept[k]) for k, v in m.state_dict().items())
+    # names and groupings that are decoded alike
+    host_linear(bits=3, fmt="int3").load_state_dict(host_linear().state_dict())
+    host_linear(group=None).load_state_dict(host_linear(group=-1).state_dict())
+    host_linear(group=128).load_state_dict(host_linear(group=None).state_dict())
+    # in a model, through a file, and from one that says nothing
+    model = nn.Sequential(host_linear(), host_linear())
+    file = io.BytesIO()
+    torch.save(model.state_dict(), file)
+    file.seek(0)
+    state = torch.load(file, weights_only=True)
+    model.load_state_dict(state)
+    assert set(state) == {f"{i}.{b}" for i in (0, 1) for b in BUFFERS + ("bias", "weight_format")}
+    with pytest.raises(RuntimeError, match="format"):
+        nn.Sequential(host_linear(), host_linear(fmt="fp4")).load_state_dict(state)
+    bare = {k: v for k, v in state.items() if not k.endswith("format")}
+    with pytest.warns(UserWarning, match="format"):
+        model.load_state_dict(bare)
+    with pytest.raises(RuntimeError, match="spare"):     # strictness is as it was
+        model.load_state_dict(dict(state, **{"0.spare": torch.zeros(1)}))
+    assert "weight_format" not in dict(model.named_buffers())
