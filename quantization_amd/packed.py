@@ -88,6 +88,21 @@ def _kind_of(wq_bits, datatype):
     return TABLE, table_order(TABLE_LISTS[datatype] if datatype in TABLE_LISTS else lut_values(datatype))
 
 
+def _check_codes(q, kind, values):
+    """Refuses codes that four bits of the kind do not hold (the library keeps them within its range, mq_w4_pack)."""
+    if kind in (INT_ASYM, INT_SYM):
+        low, high = (0, 15) if kind == INT_ASYM else (-7, 7)
+        lo, hi = torch.aminmax(q.view(torch.uint8 if kind == INT_ASYM else torch.int8))
+        if int(lo) < low or int(hi) > high:
+            raise ValueError(f"codes from {int(lo)} to {int(hi)}: {low} to {high} can be packed")
+        return
+    known = torch.zeros_like(q, dtype=torch.bool)
+    for v in sorted(set(lut_values("fp4") if kind == FP4 else values)):
+        known |= q == v
+    if not bool(known.all()):
+        raise ValueError("codes that are not values of the table")
+
+
 def _group(group_size):
     """quant_weight.py:241-255: > 0 per group, -1 per tensor, everything else per row."""
     if group_size is None or (group_size <= 0 and group_size != -1):
@@ -187,9 +202,14 @@ def _dequantize(weight):
 def pack_codes(q, scale, zp=None, wq_bits: int = 4, datatype: str = "int4", group_size=None) -> PackedWeight:
     """Pack codes and parameters as _int_quant_meta / _fp_quant_meta return them (quant_weight.py:717-872).
 
-    q: int8 / uint8 codes (integers) or float16 table values, [N, K] or [N, G, group_size]; scale (and, for asymmetric
-    integers, zp): float16, [N, G] per group, [N] per row, [] per tensor.  With a leading dimension E on all of them: a
-    stack of experts.  Groups are multiples of 32 that divide K; rows may have any length."""
+    q: int8 / uint8 codes (integers: 0 .. 15 with zero points, -7 .. 7 without) or float16 table values, [N, K] or
+    [N, G, group_size]; scale (and, for asymmetric integers, zp): float16, [N, G] per group, [N] per row, [] per tensor.
+    With a leading dimension E on all of them: a stack of experts.  Groups are multiples of 32 that divide K; rows may have
+    any length.  Codes that the format does not hold raise ValueError (which waits for the device)."""
+    return _pack(q, scale, zp, wq_bits, datatype, group_size, True)
+
+
+def _pack(q, scale, zp, wq_bits, datatype, group_size, check):
     if _compiling() or _tracing() or get_proxy_mode() is not None:
         raise RuntimeError("packing a weight cannot be recorded: pack it beforehand")
     kind, values = _kind_of(wq_bits, datatype)
@@ -218,6 +238,8 @@ def pack_codes(q, scale, zp=None, wq_bits: int = 4, datatype: str = "int4", grou
     if q.dtype not in ((torch.float16,) if kind >= TABLE else (torch.int8, torch.uint8)):
         raise ValueError(f"codes of {datatype} cannot be {q.dtype}")
     q = require_device(q).contiguous()
+    if check:
+        _check_codes(q, kind, values)
     dev = q.device
 
     def rows(t):   # one scale per row at least
@@ -283,7 +305,7 @@ def pack_weight(w, wq_bits: int = 4, datatype: str = "int4", group_size=None) ->
         q, scale, zp = meta(w.reshape(e * n, k))
         q, scale = q.reshape(e, n, k), scale.reshape((e, n) + tuple(scale.shape[1:]))
         zp = None if zp is None else zp.reshape(scale.shape)
-    return pack_codes(q, scale, zp, wq_bits, datatype, group_size)
+    return _pack(q, scale, zp, wq_bits, datatype, group_size, False)
 
 
 def _rows_of(t):

@@ -204,3 +204,24 @@ def test_a_state_dict_of_another_format_is_refused(pk):
     again = layer(pk, seed=1)
     again.load_state_dict({k: v.cpu() for k, v in m.state_dict().items()})
     assert torch.equal(again(x), want)
+
+
+def test_packing_refuses_codes_that_it_would_change(pk):
+    s = torch.ones(8, 2, dtype=torch.float16, device="cuda")
+    q = torch.randint(-7, 8, (8, 64), dtype=torch.int8, device="cuda")
+    assert torch.equal(pk.pack_codes(q, s, group_size=32).dequantize(), q.half())
+    for v in (-8, 8):
+        q[3, 5] = v
+        with pytest.raises(ValueError):
+            pk.pack_codes(q, s, group_size=32)
+    u = torch.randint(0, 16, (8, 64), dtype=torch.uint8, device="cuda")
+    assert torch.equal(pk.pack_codes(u, s, s, datatype="int4_asym", group_size=32).dequantize(), u.half() - 1)
+    u[0, 0] = 16
+    with pytest.raises(ValueError):
+        pk.pack_codes(u, s, s, datatype="int4_asym", group_size=32)
+    t = torch.tensor([0, 1, 2, 3, 4, 6, 8, 12], device="cuda").half().repeat(8, 8)
+    assert torch.equal(pk.pack_codes(t, s, datatype="fp4", group_size=32).dequantize(), t)
+    for v in (5, float("nan"), 16):
+        t[7, 63] = v
+        with pytest.raises(ValueError):
+            pk.pack_codes(t, s, datatype="fp4", group_size=32)
