@@ -261,11 +261,15 @@ def quant_model(model, wq_bits: Optional[int] = None, wq_datatype: Optional[str]
     if packed:
         from .packed import PackedLinear, _kind_of
         _kind_of(wq_bits, wq_datatype)
+        if isinstance(model, nn.Linear):
+            raise ValueError("a Linear that is the model itself cannot be swapped in it: use PackedLinear(model, ...)")
         print(f"Packing weights in 4 bits: {wq_bits}-bit {wq_datatype}, group size: {wq_groupsize}")
-        linears = [(name, PackedLinear(m, wq_bits, wq_datatype, wq_groupsize)) for name, m in _linears(model)]
-        for name, mod in linears:   # (only once every weight has been packed: a refused one leaves the model as it was)
-            parent, attr = _find_parent(model, name)
-            setattr(parent, attr, mod)
+        linears = {m: PackedLinear(m, wq_bits, wq_datatype, wq_groupsize) for _, m in _linears(model)}
+        # (only once every weight has been packed: a refused one leaves the model as it was; a shared one in all its places)
+        for name, m in list(model.named_modules(remove_duplicate=False)):
+            if m in linears:
+                parent, attr = _find_parent(model, name)
+                setattr(parent, attr, linears[m])
         return
     if wq_datatype.startswith("int"):
         asym = "asym" in wq_datatype

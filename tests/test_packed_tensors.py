@@ -13,6 +13,7 @@ from torch.autograd import forward_ad as fa
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from quantization_amd import packed
+from quantization_amd.quant_weight import quant_model
 
 
 class StandIn:
@@ -291,3 +292,24 @@ def test_codes_that_the_format_does_not_hold_are_refused():
                     (16, packed.FP4), (0.5, packed.FP4), (float("nan"), packed.FP4)):
         with pytest.raises(ValueError, match="codes"):
             check(torch.tensor([[1, 2], [v, 0]]).half(), kind, values)
+
+
+def test_quant_model_packs_a_shared_layer_in_all_its_places(host_linear):
+    class Twice(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.down = nn.Linear(128, 128)
+            self.again = self.down
+            self.blocks = nn.ModuleList([nn.Sequential(nn.Linear(128, 32), self.down)])
+            self.blocks.append(self.blocks[0])
+
+    m = Twice()
+    quant_model(m, wq_bits=4, wq_datatype="int4", wq_groupsize=64, packed=True)
+    assert isinstance(m.down, packed.PackedLinear) and isinstance(m.blocks[0][0], packed.PackedLinear)
+    assert m.down is m.again is m.blocks[0][1] and m.blocks[0] is m.blocks[1]
+    assert not [x for x in m.modules() if isinstance(x, nn.Linear)]
+    # nothing holds a Linear that is the model itself: it cannot be swapped
+    root = nn.Linear(128, 32)
+    with pytest.raises(ValueError, match="PackedLinear"):
+        quant_model(root, wq_bits=4, wq_datatype="int4", wq_groupsize=64, packed=True)
+    assert list(root.named_children()) == []
