@@ -657,7 +657,8 @@ size_t mq_w4_params_bytes(const mq_w4* w);                       /* 0: refused (
  * +-7 stands for +-7) or float16 table values (TABLE, FP4; a value that is not in the table stands for 0); scale, zero:
  * float16 [experts][n][k / group or 1], zero only with INT_ASYM. */
 int mq_w4_pack(const mq_w4* w, const void* codes, const void* scale, const void* zero, void* hip_stream);
-/* deq float16 [experts][n][k] = h(h(q - zero) * scale): the bits that the quantizers' own deq output has. */
+/* deq float16 [experts][n][k] = h(h(q - zero) * scale): the bits that the quantizers' own deq output has (f32_math = 0),
+ * but for the sign of zero. */
 int mq_w4_unpack(const mq_w4* w, void* deq, void* hip_stream);
 
 /* May be 0.  aligned: every row of x (dy) starts on a multiple of 16 bytes and the next one at most 2^23 elements on;

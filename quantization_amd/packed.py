@@ -180,7 +180,9 @@ class PackedWeight:
 
     @torch.no_grad()
     def dequantize(self):
-        """The float16 weight, with the bits that quant_int / quant_int_asym / quant_datatype return for it."""
+        """The float16 weight, with the bits that _int_quant_meta / _fp_quant_meta return for it, but for the sign of zero
+        (a code has none): those of quant_int, quant_int_asym and quant_datatype too, except for a table with one scale per
+        tensor, which quant_datatype computes in float32 (quant_weight.py:562-575)."""
         if _recorded(self.data):
             tensors, form = self._operands()
             return torch.ops.quantization_amd.packed_dequantize(*tensors, *form)

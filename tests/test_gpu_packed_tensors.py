@@ -225,3 +225,21 @@ def test_packing_refuses_codes_that_it_would_change(pk):
         t[7, 63] = v
         with pytest.raises(ValueError):
             pk.pack_codes(t, s, datatype="fp4", group_size=32)
+
+
+@pytest.mark.parametrize("fmt,bits", [("fp4", 4), ("flint4", 4), ("fp4_er_pos", 4), ("fp4_ea_neg", 4), ("fp3", 3), ("int4", 4),
+                                      ("int4_asym", 4)])
+def test_dequantize_with_one_scale_per_tensor(pk, fmt, bits):
+    """The bits of the quantizers' dequantized weight (for tables not quant_datatype's, which are float32 arithmetic's)."""
+    from quantization_amd import quant_weight as qw
+    torch.manual_seed(3)
+    w = (torch.randn(200, 320, device="cuda") * 0.02).half()
+    got = pk.pack_weight(w, bits, fmt, -1).dequantize()
+    if fmt.startswith("int"):
+        want, again = qw._int_quant_meta(w, bits, "asym" in fmt, -1)[0], qw.quant_int_asym if "asym" in fmt else qw.quant_int
+        again = again(w, bits, -1)
+    else:
+        want, again = qw._fp_quant_meta(w, bits, fmt, -1)[0], None
+    bits_of = lambda t: torch.where(t == 0, 0, t.view(torch.int16))
+    assert torch.equal(bits_of(got), bits_of(want))
+    assert again is None or torch.equal(bits_of(got), bits_of(again))
