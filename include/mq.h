@@ -622,9 +622,13 @@ int mq_histogram(const void* x, int32_t dtype, int64_t n, const double* edges, i
  *
  * x, dy, bias: float16 or bfloat16, y / dx of the same type, sums in float32, one rounding at the end.  In mq_linear4
  * the codes' values enter the matrix cores exactly and the scales are applied in float32.  In mq_linear4_grad the scales
- * change along the sum, so each weight is rounded once to float16 (by 2^-11 of it at most); rows of bfloat16 are brought
- * into float16's range by a power of two each, exactly but for values more than 2^28 below their row's largest.  With zero points the sum is taken as scale * sum(q x) - scale * zero * sum(x): an infinite x[r][k] makes
- * the whole row NaN where (q - zero) x would have left infinities.
+ * change along the sum, so each weight is held in float16, times a power of two per expert (norm): it is off by at most
+ * 2^-11 |W| + 2^-39 (|q - zero| + 1) T, T the expert's largest |scale| times 16 (with zero points: times 15 + the largest
+ * |zero|; and where q - zero is no float16 number itself, which takes a |zero| above 2048 or one that is no integer, by
+ * 2^-11 |W| more).  Rows of bfloat16 are brought into float16's range by a power of two each, exactly but for values more than
+ * 2^28 below their row's largest, which are off by 2^-39 of that at most.  With zero points the sum is taken as
+ * scale * sum(q x) - scale * zero * sum(x): an infinite x[r][k] makes the whole row NaN where (q - zero) x would have left
+ * infinities.
  *
  * Rows and experts: counts == NULL: one weight (experts == 1) for all rows.  Otherwise the rows are sorted by expert and
  * counts (DEVICE, int32 [experts]) says how many each has, none included; the host never reads it.  Counts below zero
@@ -643,7 +647,8 @@ typedef struct {
   const void* data;   /* DEVICE, 16-byte aligned, mq_w4_data_bytes: codes in tiles of 16 rows x 128 columns      */
   const void* params; /* DEVICE, 16-byte aligned, mq_w4_params_bytes: scales (and zero points) per tile row      */
   const float* norm;  /* DEVICE [experts]: a power of two that brings an expert's largest |weight| near 2^15; the
-                         gradient's float16 weights are held times it so that small scales keep their bits       */
+                         gradient's float16 weights are held times it so that small scales keep their bits: those of
+                         2^-23 of the largest and more do (with zero points of up to 15)                         */
   int64_t experts, n, k;
   int64_t group;      /* columns per scale: a multiple of 32 that divides k, or 0 = one per row (any k)          */
   int32_t kind;       /* mq_w4_kind */

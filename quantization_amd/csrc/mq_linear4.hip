@@ -275,7 +275,7 @@ template <int KIND> __global__ __launch_bounds__(64) void k_w4_turn(const W4Args
         }
       }
       const int64_t to = (e * a.gp + grp) * t.rb * 128 + n;
-      t.ts[to] = W4F16::from_f32(s * up);  // exact, but for scales more than 2^25 below the expert's largest
+      t.ts[to] = W4F16::from_f32(s * up);  // exact down to 2^-14, off by 2^-25 at most below
       if constexpr (KIND == W4_U4) t.tz[to] = W4F16::from_f32(z);
     }
   }

@@ -215,8 +215,9 @@ __global__ __launch_bounds__(MT * NT == 1 ? 1024 : 512) void k_w4_rows(const W4A
 
 // ---- the gradient's scaled weights ---------------------------------------------------------------------
 // Eight weights of one column in float16, scale * (q - zero) times the expert's norm (a power of two): the difference is
-// exact for zero points up to 2048 (beyond it rounds as the quantizers' dequantization does), the product rounds once (2^-11
-// of the weight at most).
+// exact for whole zero points up to 2048 (others round it by 2^-11 of itself, as the quantizers' dequantization does), the
+// product rounds once: by 2^-11 of the weight, or 2^-25 where it is below 2^-14, 2^-28 or less of what the expert's largest
+// scale can make.
 template <int KIND> struct W4Scales {
   u32x4 s, z;
   __device__ __forceinline__ u32x4 scaled(uint32_t d, const W4Lut& lut) const {
