@@ -69,3 +69,41 @@ def test_gradient_where_the_scales_are_far_apart(pk, fmt, dtype):
             got = gradient(pk, p, dy).double()
             bad = ((got - want).abs() > tol) & fits
             assert not bad.any(), (low, high, m, int(bad.sum()), float(((got - want).abs() / tol)[fits].max()))
+
+
+def runs(rows, experts=1):
+    """Into how many runs the rows' sum is cut: up to 512 rows of an expert, on average, in one."""
+    per = rows // experts
+    return 1 if per <= 512 else min(per // 256, 32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_bias_gradient_adds_every_row_once(pk, dtype):
+    """db = sum of dy over the rows.  A run's rows are added by sixteen waves in turn, the waves' sums and the runs' one after
+    the other: a term passes at most rows / (16 runs) + 1 + 15 + runs float32 additions.  Whole numbers whose sums stay below
+    2^24 are added without any rounding."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    n, k = 70, 64
+    p = pk.pack_weight(torch.randn(n, k, generator=gen, device="cuda").half(), 4, "int4", 32)
+    pe = pk.pack_weight(torch.randn(3, n, k, generator=gen, device="cuda").half(), 4, "int4", 32)
+    eps = torch.finfo(dtype).eps / 2
+    for m in (1, 15, 16, 17, 300, 512, 513, 767, 768, 1000, 1537, 5000, 9000, 20000):
+        x = torch.zeros(m, k, device="cuda", dtype=dtype)
+        counts = torch.tensor([m // 2, 0, m - m // 2 - m // 7], device="cuda")
+        ends = [0, m // 2, m // 2, m - m // 7]
+        real = torch.randn(m, n, generator=gen, device="cuda").to(dtype)
+        whole = torch.randint(-8, 9, (m, n), generator=gen, device="cuda").to(dtype)
+        for dy in (real, whole):
+            b = torch.zeros(n, dtype=dtype, device="cuda", requires_grad=True)
+            be = torch.zeros(3, n, dtype=dtype, device="cuda", requires_grad=True)
+            got, = torch.autograd.grad(pk.packed_linear(x, p, b), b, dy)
+            some, = torch.autograd.grad(pk.packed_expert_linear(x, pe, counts, be), be, dy)
+            for part, d, r in [(got, dy, runs(m))] + [(some[e], dy[ends[e]:ends[e + 1]], runs(m, 3)) for e in range(3)]:
+                want = d.double().sum(0)
+                if dy is whole:
+                    assert torch.equal(part, want.to(dtype)), m
+                    continue
+                depth = math.ceil(len(d) / (16 * r)) + 16 + r
+                tol = eps * want.abs() + depth * 2.0 ** -24 * (1 + 2 * eps) * d.double().abs().sum(0)
+                off = (part.double() - want).abs()
+                assert not (off > tol).any(), (m, float((off / tol).max()))
