@@ -626,7 +626,9 @@ int mq_histogram(const void* x, int32_t dtype, int64_t n, const double* edges, i
  * 2^-11 |W| + 2^-39 (|q - zero| + 1) T, T the expert's largest |scale| times 16 (with zero points: times 15 + the largest
  * |zero|; and where q - zero is no float16 number itself, which takes a |zero| above 2048 or one that is no integer, by
  * 2^-11 |W| more).  Rows of bfloat16 are brought into float16's range by a power of two each, exactly but for values more than
- * 2^28 below their row's largest, which are off by 2^-39 of that at most.  With zero points the sum is taken as
+ * 2^28 below their row's largest, which are off by 2^-39 of that at most.  In mq_linear4 the sums over up to 128 code values
+ * come before the scales, in float32: bfloat16 activations from 2^116 on can overflow there (with zero points the product
+ * scale * zero * sum(x) as well) although the result would be finite.  With zero points the sum is taken as
  * scale * sum(q x) - scale * zero * sum(x): an infinite x[r][k] makes the whole row NaN where (q - zero) x would have left
  * infinities.
  *

@@ -8,7 +8,8 @@ layout that the matrix-core kernels read (include/mq.h, mq_w4 / mq_linear4), and
   PackedLinear                                       nn.Linear's place in a model (quant_model(..., packed=True))
 
 W = scale * (q - zero point), per group of input channels; the weight is frozen (no gradient for codes or scales).
-Activations are float16 or bfloat16, sums float32, results rounded once.  The reference keeps such codes beside the weight
+Activations are float16 or bfloat16 (below 2^116: sums over code values come before the scales), sums float32, results
+rounded once.  The reference keeps such codes beside the weight
 (_LinearDump, quant_weight.py:876-914) and multiplies by the dequantized float16 weight; there is no CPU compute path.
 """
 import ctypes

@@ -107,3 +107,18 @@ def test_bias_gradient_adds_every_row_once(pk, dtype):
                 tol = eps * want.abs() + depth * 2.0 ** -24 * (1 + 2 * eps) * d.double().abs().sum(0)
                 off = (part.double() - want).abs()
                 assert not (off > tol).any(), (m, float((off / tol).max()))
+
+
+def test_rows_of_large_and_small_activations(pk):
+    """Forward, the sums run over code values before the scales come in: a sum of 128 values of up to 16 times an activation
+    has to stay in float32, so activations below 2^116 do, and results are right wherever they themselves fit."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    n, k, g = 96, 512, 128
+    for fmt in ("int4", "int4_asym", "flint4"):
+        p = pk.pack_weight((torch.randn(n, k, generator=gen, device="cuda") * 0.02).half(), 4, fmt, g)
+        unit = torch.randn(300, k, generator=gen, device="cuda").clamp_(-4, 4).bfloat16()
+        for m in (3, 20, 300):
+            want = pk.packed_linear(unit[:m], p)
+            for e in (113, 60, -60, -90):
+                x = (unit[:m].double() * 2.0 ** e).bfloat16()     # a power of two: every sum is the same times 2^e
+                assert torch.equal(pk.packed_linear(x, p).double(), (want.double() * 2.0 ** e)), (fmt, m, e)
