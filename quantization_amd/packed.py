@@ -153,7 +153,10 @@ class PackedWeight:
 
     def _versions(self):
         """How often each tensor has been written in place (tensors of inference mode do not say)."""
-        return [0 if t.is_inference() else t._version for t in (self.data, self.params, self.norm)]
+        try:
+            return self.data._version, self.params._version, self.norm._version
+        except RuntimeError:
+            return None
 
     def __getstate__(self):
         return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref", "_at", "_need")}
@@ -323,17 +326,17 @@ def _rows_of(t):
 
 def _on_device(call, t, *args):
     """call(t, *args) with t's device as the current one."""
-    index = t.device.index
+    index = t.get_device()
     if index == torch._C._cuda_getDevice():
         return call(t, *args, index)
     with torch.cuda.device(index):
         return call(t, *args, index)
 
 
-def _workspace(weight, t, at, rows, ld, counts, grad):
+def _workspace(weight, t, code, at, rows, ld, counts, grad):
     """-> (tensor | None, its address, bytes).  Of this call alone: a captured graph keeps it in its own pool, and calls on
     other streams have their own."""
-    key = (_XDTYPES[t.dtype], rows, at % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 23 or rows == 1), counts is not None, grad)
+    key = (code, rows, at % 16 == 0 and (ld % 8 == 0 and ld <= 1 << 23 or rows == 1), counts is not None, grad)
     need = weight._need.get(key)
     if need is None:
         if len(weight._need) >= 4096:
@@ -347,14 +350,14 @@ def _workspace(weight, t, at, rows, ld, counts, grad):
 
 def _forward(x, weight, bias, counts, index):
     L = _bound or _bind()
-    rows = x.shape[0]
+    (rows, k), code = x.shape, _XDTYPES[x.dtype]
     y = x.new_empty((rows, weight.n))
     if rows:
         ref = weight._taken()
-        x, ld = _rows_of(x)
+        x, ld = (x, k) if x.is_contiguous() else _rows_of(x)
         at = x.data_ptr()
-        ws, wp, need = _workspace(weight, x, at, rows, ld, counts, 0)
-        rc = L.mq_linear4(ref, at, _XDTYPES[x.dtype], rows, ld, None if bias is None else bias.data_ptr(),
+        ws, wp, need = _workspace(weight, x, code, at, rows, ld, counts, 0)
+        rc = L.mq_linear4(ref, at, code, rows, ld, None if bias is None else bias.data_ptr(),
                           None if counts is None else counts.data_ptr(), y.data_ptr(), wp, need,
                           torch._C._cuda_getCurrentRawStream(index))
         if rc:
@@ -371,9 +374,9 @@ def _backward(dy, weight, counts, want_x, want_bias, index):
         return dx, None if db is None else db.zero_()
     ref = weight._taken()
     dy, ld = _rows_of(dy)
-    at = dy.data_ptr()
-    ws, wp, need = _workspace(weight, dy, at, rows, ld, counts, want_x + 2 * want_bias)
-    rc = L.mq_linear4_grad(ref, at, _XDTYPES[dy.dtype], rows, ld, None if counts is None else counts.data_ptr(),
+    at, code = dy.data_ptr(), _XDTYPES[dy.dtype]
+    ws, wp, need = _workspace(weight, dy, code, at, rows, ld, counts, want_x + 2 * want_bias)
+    rc = L.mq_linear4_grad(ref, at, code, rows, ld, None if counts is None else counts.data_ptr(),
                            None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), wp, need,
                            torch._C._cuda_getCurrentRawStream(index))
     if rc:
@@ -385,13 +388,13 @@ def _backward(dy, weight, counts, want_x, want_bias, index):
 # The calls above hand addresses to the library, which nothing in torch sees: a recorder would keep the allocation of the
 # result alone and replay that.  So wherever one is at work the same calls run as operators of torch's own.
 _PLAIN = {torch.Tensor, nn.Parameter, type(None)}
-_compiling, _tracing, _modes = torch.compiler.is_compiling, torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+_compiling, _tracing, _modes = torch.compiler.is_dynamo_compiling, torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 
 
 def _recorded(x, bias=None, counts=None):
     """True under torch.compile, torch.jit.trace, a dispatch mode (make_fx, torch.export, fake tensors) or for tensors of
     another class."""
-    return (_compiling() or _tracing() or _modes() > 0 or type(x) not in _PLAIN or type(bias) not in _PLAIN
+    return (_compiling() or _tracing() or _modes() or type(x) not in _PLAIN or type(bias) not in _PLAIN
             or type(counts) not in _PLAIN)
 
 
@@ -401,6 +404,8 @@ def _product_op(x: torch.Tensor, data: torch.Tensor, params: torch.Tensor, norm:
                 datatype: str) -> torch.Tensor:
     weight = PackedWeight(data, params, norm, experts or None, n, k, group_size, wq_bits, datatype)
     bias, counts = _check_operands(x, weight, bias), _check_rows(x, weight, counts)
+    if x.dim() != 2:
+        raise ValueError(f"rows [R, {k}] are wanted, got {tuple(x.shape)}")
     return _on_device(_forward, x, weight, bias, counts)
 
 
@@ -476,8 +481,10 @@ class _PackedProduct(torch.autograd.Function):
         # (the weight's tensors are not saved: hooks that move what is saved would carry the whole weight to and fro)
         ctx.weight, ctx.versions = weight, weight._versions()
         ctx.save_for_backward(counts)
-        ctx.save_for_forward(counts)
-        return _product(x, weight, bias, counts)
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(counts)
+            return _product(x, weight, bias, counts)
+        return _on_device(_forward, x, weight, bias, counts)   # (_run has seen that nobody records it)
 
     @staticmethod
     @once_differentiable
@@ -506,9 +513,10 @@ def _check_operands(x, weight, bias):
         raise RuntimeError("packed products expect ROCm device tensors; no CPU fallback exists")
     if x.dtype not in _XDTYPES:
         raise ValueError(f"float16 or bfloat16 activations are wanted, got {x.dtype}")
-    if not x.dim() or x.shape[-1] != weight.k:
+    shape = x.shape
+    if not shape or shape[-1] != weight.k:
         raise ValueError(f"activations {tuple(x.shape)} do not fit a weight {tuple(weight.shape)}")
-    if x.device != weight.data.device:
+    if x.get_device() != weight.data.get_device():
         raise ValueError(f"activations on {x.device}, weight on {weight.device}")
     if bias is not None:
         want = (weight.n,) if weight.experts is None else (weight.experts, weight.n)
@@ -550,8 +558,9 @@ def packed_linear(x, weight: PackedWeight, bias=None):
     bias = _check_operands(x, weight, bias)
     if weight.experts is not None:
         raise ValueError("a stack of experts goes through packed_expert_linear")
-    y = _run(x if x.dim() == 2 else x.reshape(-1, weight.k), weight, bias, None)
-    return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (weight.n,))
+    if x.dim() == 2:
+        return _run(x, weight, bias, None)
+    return _run(x.reshape(-1, weight.k), weight, bias, None).reshape(x.shape[:-1] + (weight.n,))
 
 
 def packed_expert_linear(x, weight: PackedWeight, counts, bias=None):

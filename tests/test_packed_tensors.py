@@ -313,3 +313,11 @@ def test_quant_model_packs_a_shared_layer_in_all_its_places(host_linear):
     with pytest.raises(ValueError, match="PackedLinear"):
         quant_model(root, wq_bits=4, wq_datatype="int4", wq_groupsize=64, packed=True)
     assert list(root.named_children()) == []
+
+
+def test_rows_of_another_shape_never_reach_the_library(launches):
+    w = host_weight()
+    for shape in ((128,), (2, 3, 128)):
+        with pytest.raises(ValueError):
+            run(torch.zeros(shape, dtype=torch.float16), w)
+    assert not launches.seen
