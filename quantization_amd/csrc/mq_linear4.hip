@@ -437,8 +437,9 @@ W4Plan plan_of(const mq_w4* w, int64_t rows, bool grad, bool counted, W4Product*
   // by what was measured on 4096 x 4096, microseconds per block of 128 for a compute unit with one tile (two sets of waves
   // in it), with two, and for an odd one behind pairs.  64 x 128 (always two sets): 0.65, 1.3, 0.55 (gradient 0.75, 1.2,
   // 0.6), 128 x 128: 1.05, 1.85, 1.2, the gradient's 128 x 256: 2.1, 3.6, 1.75 (one tile with one set of waves: forward
-  // 1.1, gradient the same without zero points and 2.4 with them; pairs with two sets: 2.15 and 4.1).  A tile begins and ends in 1.5; a join takes 3 and moves its
-  // sums at about 4 MB per microsecond.
+  // 1.1, gradient the same without zero points and 2.4 with them; pairs with two sets: 2.15 and 4.1).  A tile begins and ends
+  // in 1.5; a join takes 3 and moves its sums at about 4 MB per microsecond.  Measured with integer codes and taken for all
+  // kinds (a table's decoding takes 19 instructions, an integer's 7).
   static const double kTime[2][2][3] = {{{0.65, 1.3, 0.55}, {1.05, 1.85, 1.2}}, {{0.75, 1.2, 0.6}, {2.1, 3.6, 1.75}}};
   double best = 0;
   for (int tall = 0; tall < 2; ++tall) {

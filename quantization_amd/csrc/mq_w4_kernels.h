@@ -55,8 +55,9 @@ template <class T> __device__ __forceinline__ void w4_store4(uint16_t* y, int64_
 // wave keeps D blocks in flight while it works on the D before them.  Rows that are not there repeat the tile's last one
 // (their loads fall into the same lines, their results are not stored; masking them off measured slower).  Rows are 16-byte
 // aligned and a multiple of 128 long (k_w4_pad).
-// Bound by reading the weight: 5 rows through 128256 x 4096 (280 MB) 48 us, 5.8 TB/s; one row through 14336 x 4096 with
-// zero points (31 MB) 9.0 us, 3.5 TB/s; 2048 x 2048 3.9 us, which is the latency of a launch and of two blocks.
+// Bound by reading the weight: 5 rows through 128256 x 4096 (280 MB) 48 us, 5.8 TB/s (a stream of reads alone reaches 7.0);
+// one row through 14336 x 4096 with zero points (31 MB) 9.3 us alone, 8.5 among others, 3.7 TB/s; 2048 x 2048 4.0 us, which
+// is the latency of a launch and of two blocks.
 template <class T, int KIND, int MT, int NT, int FS, int D> struct W4RowsStage {
   u32x4 w[D][NT], x[D][MT][4];
   uint32_t s[D][NT];  // lane 16 v + c: the scale (and zero point) of column c in window v of the block's 4 / FS
@@ -250,7 +251,8 @@ template <int KIND> struct W4Scales {
 // to 218).  Zero points: minus (scale * zero)[column] * (sum of x)[row] per window of FS steps, a float32 product on the
 // matrix cores with a contraction over the windows (v_mfma_f32_32x32x2_f32): the vector units took as many instructions
 // for it as for the scaling (2048 x 4096 x 4096, groups of 64: 106 us, 100 with the product).
-// 2000 rows through 14336 x 4096: 218 us, 1.08 PFLOP/s.  The matrix cores are busy in 0.59 of the cycles, 168 vector
+// 2000 rows through 14336 x 4096: 199 to 214 us a call, by the card, 1.10 to 1.18 PFLOP/s (the times of the steps above are
+// launches kept apart by a profiler, 206 to 218 us now).  The matrix cores are busy in 0.58 of the cycles, 168 vector
 // instructions stand beside every 32 products, and under this load the clock falls to 1.8 GHz: the steps above took 11 % of
 // the cycles away and 4 % of the time.
 //
@@ -260,7 +262,12 @@ template <int KIND> struct W4Scales {
 // as much error as the rounding of the result (2.4e-3 of the norm against 1.7e-3) and take more instructions to make.  The
 // scales along the contraction come with the block's rows through LDS, two to a lane (4096 x 4096 x 4096: 131 us, 149 with
 // loads between the products).  2048 rows through 4096 x 4096, one tile to a compute unit: 83 us with zero points, the matrix
-// cores busy in 0.35 of the cycles, the waves waiting for loads in 0.33; 4096 rows without: 1.05 PFLOP/s, turning included.
+// cores busy in 0.35 of the cycles, the waves waiting in 0.33; 4096 rows without: 1.05 PFLOP/s, turning included.  What bounds
+// that tile of 128 x 256 are its instructions: with zero points 386 vector ones stand beside every 64 products (float16 rows),
+// the subtraction q - zero being compiled value by value, 12 instructions where 4 would do; and for rows of bfloat16 (475) the
+// compiler does not see that the tile's place is the same in all lanes, keeps the buffer descriptors in vector registers and
+// puts each of the block's 14 to 16 loads into a loop over their values.  With two sets of waves 76 bytes a lane are spilled,
+// outside the loop.
 template <int NT, int W> struct W4Ahead {  // what a wave holds of a block that is on its way
   u32x4 b[NT][2];
   uint32_t s[NT][W];
@@ -313,7 +320,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_w4_gemm(const W4Args a
 
   if (expert >= 0) {
     // 16-row tile of this lane's row: tiles past the end repeat the last one (their results are not stored)
-    // The loads go through buffer descriptors: one offset per lane for the whole loop, the block's in a scalar register.
+    // The loads go through buffer descriptors: one offset per lane for the whole loop, the block's in a scalar register.  (The
+    // descriptors are scalar too but in the gradient's large tile with a bfloat16 result: see above.)
     const int64_t bt0 = (tile0 - wn * NT) * 2 < p.ct ? (tile0 - wn * NT) * 2 : p.ct - 1;  // the workgroup's first 16-row tile
     const auto bsrc = w4_buffer(p.b + ((int64_t)expert * p.ct + bt0) * p.rb * 256, (uint32_t)(WN * NT * 2) * (uint32_t)p.rb * 1024u);
     const auto xsrc = w4_buffer(p.x + row0 * p.ldx, (uint32_t)(((int64_t)(rows - 1) * p.ldx + (int64_t)p.rb * 128) * 2));
