@@ -637,13 +637,14 @@ class PackedLinear(nn.Module):
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
         key = prefix + "weight_format"
-        if key in state_dict:
-            theirs = bytes(state_dict[key].tolist()).decode(errors="replace")
+        text = state_dict.get(key)
+        if text is not None and not text.is_meta:
+            theirs = bytes(text.to(torch.uint8).tolist()).decode(errors="replace")
             if theirs != self._format():   # nothing of it is taken over
                 error_msgs.append(f"{key}: the format of the state dict's weight is \"{theirs}\", this module's "
                                   f"\"{self._format()}\"")
                 return
-        elif prefix + "weight_data" in state_dict:
+        elif text is None and prefix + "weight_data" in state_dict:
             warnings.warn(f"{key} is missing: a weight of another format would be decoded wrongly", stacklevel=2)
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
         if key in unexpected_keys:

@@ -321,3 +321,14 @@ def test_rows_of_another_shape_never_reach_the_library(launches):
         with pytest.raises(ValueError):
             run(torch.zeros(shape, dtype=torch.float16), w)
     assert not launches.seen
+
+
+def test_formats_in_other_clothes(host_linear):
+    """A text of another integer type is read; one without contents (meta tensors) says nothing."""
+    m = host_linear()
+    state = dict(m.state_dict())
+    state["weight_format"] = state["weight_format"].long()
+    m.load_state_dict(state)
+    meta = {k: v.to("meta") for k, v in state.items()}
+    m.load_state_dict(meta, assign=True)
+    assert m.weight_data.is_meta
