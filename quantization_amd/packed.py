@@ -403,6 +403,7 @@ def _product_op(x: torch.Tensor, data: torch.Tensor, params: torch.Tensor, norm:
                 counts: Optional[torch.Tensor], experts: int, n: int, k: int, group_size: int, wq_bits: int,
                 datatype: str) -> torch.Tensor:
     weight = PackedWeight(data, params, norm, experts or None, n, k, group_size, wq_bits, datatype)
+    _no_tangents(x, bias)
     bias, counts = _check_operands(x, weight, bias), _check_rows(x, weight, counts)
     if x.dim() != 2:
         raise ValueError(f"rows [R, {k}] are wanted, got {tuple(x.shape)}")
@@ -419,6 +420,7 @@ def _gradient_op(dy: torch.Tensor, data: torch.Tensor, params: torch.Tensor, nor
                  counts: Optional[torch.Tensor], experts: int, n: int, k: int, group_size: int, wq_bits: int, datatype: str,
                  want_x: bool, want_bias: bool) -> Tuple[torch.Tensor, torch.Tensor]:
     """What is not wanted comes back empty."""
+    _no_tangents(dy)
     weight = PackedWeight(data, params, norm, experts or None, n, k, group_size, wq_bits, datatype)
     if dy.dtype not in _XDTYPES or dy.dim() != 2 or dy.shape[1] != n or dy.device != data.device:
         raise ValueError(f"a gradient {dy.dtype} {tuple(dy.shape)} on {dy.device} does not fit a weight {tuple(weight.shape)}")
@@ -475,6 +477,17 @@ def _gradient(dy, weight, counts, want_x, want_bias):
     return _on_device(_backward, dy, weight, counts, want_x, want_bias)
 
 
+def _solid(t):
+    """t in memory: tangents may be zeros without any."""
+    return torch.zeros(t.shape, dtype=t.dtype, device=t.device) if t._is_zerotensor() else t
+
+
+def _no_tangents(*tensors):
+    """The operators have no forward-mode formula; torch would drop the tangents without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("forward-mode differentiation goes through packed_linear and packed_expert_linear")
+
+
 class _PackedProduct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, weight, counts):
@@ -494,16 +507,18 @@ class _PackedProduct(torch.autograd.Function):
         if want_x and ctx.weight._versions() != ctx.versions:
             raise RuntimeError("the packed weight has been written in place since the forward pass: its gradient would be "
                                "that of another weight")
+        dy, tangent = (dy, None) if forward_ad._current_level < 0 else forward_ad.unpack_dual(dy)
         dx, db = _gradient(dy, ctx.weight, counts, want_x, want_bias)
+        if tangent is not None:   # (linear in dy)
+            tx, tb = _gradient(_solid(tangent), ctx.weight, counts, want_x, want_bias)
+            dx, db = (None if v is None else forward_ad.make_dual(v, t) for v, t in ((dx, tx), (db, tb)))
         return dx, db, None, None
 
     @staticmethod
     def jvp(ctx, dx, dbias, *_):
         """Linear in x and the bias: the tangent is the product of the tangents."""
         counts, = ctx.saved_tensors
-        if dx._is_zerotensor():   # (one without memory)
-            dx = torch.zeros(dx.shape, dtype=dx.dtype, device=dx.device)
-        return _run(dx, ctx.weight, dbias, counts)
+        return _run(_solid(dx), ctx.weight, None if dbias is None else _solid(dbias).contiguous(), counts)
 
 
 def _check_operands(x, weight, bias):

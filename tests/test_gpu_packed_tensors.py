@@ -243,3 +243,41 @@ def test_dequantize_with_one_scale_per_tensor(pk, fmt, bits):
     bits_of = lambda t: torch.where(t == 0, 0, t.view(torch.int16))
     assert torch.equal(bits_of(got), bits_of(want))
     assert again is None or torch.equal(bits_of(got), bits_of(again))
+
+
+def test_second_derivatives_forward_over_reverse(pk):
+    """A Hessian times a vector: of f(x) = sum(y^2) / 2, y = x W^T + b, it is (v W^T) W."""
+    w = layer(pk).packed
+    b = torch.randn(96, device="cuda").half()
+    x = (torch.randn(40, 256, device="cuda") * 0.1).half().requires_grad_()
+    v = (torch.randn(40, 256, device="cuda") * 0.1).half()
+    with fa.dual_level():
+        y = pk.packed_linear(fa.make_dual(x, v), w, b)
+        at, moves = fa.unpack_dual(y)
+        dx, = torch.autograd.grad(y, x, fa.make_dual(at.detach(), moves.detach()))     # (detach alone would drop the tangent)
+        primal, tangent = fa.unpack_dual(dx)
+    with torch.no_grad():
+        yv = pk.packed_linear(v, w)
+    z = torch.zeros_like(x, requires_grad=True)
+    assert torch.equal(primal, torch.autograd.grad(pk.packed_linear(z, w), z, pk.packed_linear(x, w, b).detach())[0])
+    assert torch.equal(tangent, torch.autograd.grad(pk.packed_linear(z, w), z, yv)[0])
+
+
+def test_the_operators_keep_torchs_rules(pk):
+    """Schema, shapes and types without data, gradients and their recording, as torch checks its own operators."""
+    tests = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+    for bias in (False, True):
+        tensors, form = layer(pk, fmt="int4_asym").packed._operands()
+        x = torch.randn(5, 256, device="cuda").half().requires_grad_()
+        b = torch.randn(96, device="cuda").half().requires_grad_() if bias else None
+        torch.library.opcheck(pk._product_op, (x, *tensors, b, None, *form), test_utils=tests)
+        torch.library.opcheck(pk._gradient_op, (torch.randn(5, 96, device="cuda").half(), *tensors, None, *form, True, bias),
+                              test_utils=tests)
+    stack = pk.pack_weight(torch.randn(3, 96, 256, device="cuda").half(), 4, "fp4", 64)
+    tensors, form = stack._operands()
+    c = torch.tensor([2, 0, 2], device="cuda", dtype=torch.int32)
+    be = torch.randn(3, 96, device="cuda").half().requires_grad_()
+    torch.library.opcheck(pk._product_op, (x, *tensors, be, c, *form), test_utils=tests)
+    torch.library.opcheck(pk._gradient_op, (torch.randn(5, 96, device="cuda").half(), *tensors, c, *form, True, True),
+                          test_utils=tests)
+    torch.library.opcheck(pk._dequantize_op, (*tensors, *form), test_utils=tests)

@@ -20,7 +20,7 @@ class StandIn:
     """libmq.so with launches that only note the addresses of the weight and the rows; sizes come from the library itself."""
 
     def __init__(self, real):
-        self.real, self.seen, self.rows = real, [], []
+        self.real, self.seen, self.rows, self.bias = real, [], [], []
 
     def __getattr__(self, name):
         return getattr(self.real, name)
@@ -31,7 +31,8 @@ class StandIn:
         self.seen.append((c.data, c.params, c.norm))
         return 0
 
-    def mq_linear4(self, ref, x, *args):
+    def mq_linear4(self, ref, x, dtype, rows, ld, bias, *args):
+        self.bias.append(bias)
         return self._note(ref, x)
 
     def mq_linear4_grad(self, ref, dy, *args):
@@ -321,6 +322,30 @@ def test_rows_of_another_shape_never_reach_the_library(launches):
         with pytest.raises(ValueError):
             run(torch.zeros(shape, dtype=torch.float16), w)
     assert not launches.seen
+
+
+def test_forward_mode_over_a_backward_pass(launches):
+    """dx and db are linear in dy: where dy has a tangent they have one, and operators called by name refuse one."""
+    w = host_weight()
+    x = rows().requires_grad_()
+    b = torch.zeros(w.n, dtype=torch.float16, requires_grad=True)
+    y = packed._run(x, w, b, None)
+    with fa.dual_level():
+        before = len(launches.seen)
+        dx, db = torch.autograd.grad(y, (x, b), fa.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        assert fa.unpack_dual(dx).tangent is not None and fa.unpack_dual(db).tangent is not None
+        assert len(launches.seen) == before + 2
+    with fa.dual_level():      # the bias's tangent is read as it lies in memory: whole rows of it
+        dual = fa.make_dual(torch.zeros(w.n, dtype=torch.float16), torch.ones(1, dtype=torch.float16).expand(w.n))
+        packed._run(rows(), w, dual, None)
+        assert launches.bias[-1] and launches.bias[-1] != launches.bias[-2]
+    tensors, form = w._operands()
+    forward, backward = packed._product_op._init_fn, packed._gradient_op._init_fn
+    with fa.dual_level():
+        with pytest.raises(NotImplementedError):
+            forward(fa.make_dual(rows(), rows()), *tensors, None, None, *form)
+        with pytest.raises(NotImplementedError):
+            backward(fa.make_dual(rows(k=32), rows(k=32)), *tensors, None, *form, True, True)
 
 
 def test_formats_in_other_clothes(host_linear):
