@@ -89,18 +89,22 @@ def _kind_of(wq_bits, datatype):
     return TABLE, table_order(TABLE_LISTS[datatype] if datatype in TABLE_LISTS else lut_values(datatype))
 
 
-def _check_codes(q, kind, values):
-    """Refuses codes that four bits of the kind do not hold (the library keeps them within its range, mq_w4_pack)."""
-    if kind in (INT_ASYM, INT_SYM):
-        low, high = (0, 15) if kind == INT_ASYM else (-7, 7)
-        lo, hi = torch.aminmax(q.view(torch.uint8 if kind == INT_ASYM else torch.int8))
-        if int(lo) < low or int(hi) > high:
-            raise ValueError(f"codes from {int(lo)} to {int(hi)}: {low} to {high} can be packed")
-        return
-    known = torch.zeros_like(q, dtype=torch.bool)
-    for v in sorted(set(lut_values("fp4") if kind == FP4 else values)):
-        known |= q == v
-    if not bool(known.all()):
+def _check_integers(q, kind):
+    """Refuses integers that four bits of the kind do not hold (the library keeps them within its range, mq_w4_pack)."""
+    low, high = (0, 15) if kind == INT_ASYM else (-7, 7)
+    lo, hi = torch.aminmax(q.view(torch.uint8 if kind == INT_ASYM else torch.int8))
+    if int(lo) < low or int(hi) > high:
+        raise ValueError(f"codes from {int(lo)} to {int(hi)}: {low} to {high} can be packed")
+
+
+def _check_values(q, c, norm, params):
+    """Refuses values that the table of c, into which q has been packed, does not hold (they became 0): unpacked with scales
+    of one, the codes have to be q."""
+    ones, out = torch.full_like(params, 0x3C00), torch.empty_like(q)
+    c.params, c.norm = ones.data_ptr(), norm.data_ptr()
+    with torch.cuda.device(q.device):
+        _lib.check(_bind().mq_w4_unpack(ctypes.byref(c), out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    if bool((out != q).any()):
         raise ValueError("codes that are not values of the table")
 
 
@@ -244,8 +248,8 @@ def _pack(q, scale, zp, wq_bits, datatype, group_size, check):
     if q.dtype not in ((torch.float16,) if kind >= TABLE else (torch.int8, torch.uint8)):
         raise ValueError(f"codes of {datatype} cannot be {q.dtype}")
     q = require_device(q).contiguous()
-    if check:
-        _check_codes(q, kind, values)
+    if check and kind < TABLE:
+        _check_integers(q, kind)
     dev = q.device
 
     def rows(t):   # one scale per row at least
@@ -275,7 +279,10 @@ def _pack(q, scale, zp, wq_bits, datatype, group_size, check):
     with torch.cuda.device(dev):
         _lib.check(L.mq_w4_pack(ctypes.byref(c), q.data_ptr(), scale.data_ptr(), None if zp is None else zp.data_ptr(),
                                 torch.cuda.current_stream().cuda_stream))
-    return PackedWeight(data, params, norm.to(torch.int32), lead[0] if experts else None, n, k, group_size, wq_bits,
+    norm = norm.to(torch.int32)
+    if check and kind >= TABLE:
+        _check_values(q, c, norm, params)
+    return PackedWeight(data, params, norm, lead[0] if experts else None, n, k, group_size, wq_bits,
                         datatype)
 
 

@@ -221,10 +221,23 @@ def test_packing_refuses_codes_that_it_would_change(pk):
         pk.pack_codes(u, s, s, datatype="int4_asym", group_size=32)
     t = torch.tensor([0, 1, 2, 3, 4, 6, 8, 12], device="cuda").half().repeat(8, 8)
     assert torch.equal(pk.pack_codes(t, s, datatype="fp4", group_size=32).dequantize(), t)
-    for v in (5, float("nan"), 16):
-        t[7, 63] = v
+    for v in (5, float("nan"), 16, float("-inf"), 0.5):
+        u = t.clone()
+        u[7, 63] = v
         with pytest.raises(ValueError):
-            pk.pack_codes(t, s, datatype="fp4", group_size=32)
+            pk.pack_codes(u, s, datatype="fp4", group_size=32)
+    from quantization_amd.fused import TABLE_LISTS
+    for fmt, bits in (("flint4", 4), ("fp4_ea_pos", 4), ("fp4_er_neg", 4), ("fp3", 3), ("fp3_ea_neg", 3)):
+        values = torch.tensor(sorted(set(TABLE_LISTS[fmt])), device="cuda").half()
+        rows = values[torch.randint(0, len(values), (2, 33, 71), device="cuda")]
+        rows[0, 0, :len(values)], rows[0, 0, 40] = values, -0.0
+        one = torch.ones(2, 33, dtype=torch.float16, device="cuda")
+        assert torch.equal(pk.pack_codes(rows, one, None, bits, fmt).dequantize(), rows)
+        for v in (-16 if fmt == "fp4_ea_pos" else 7, float("nan"), 9, 1.5):
+            bad = rows.clone()
+            bad[1, 32, 70] = v
+            with pytest.raises(ValueError):
+                pk.pack_codes(bad, one, None, bits, fmt)
 
 
 @pytest.mark.parametrize("fmt,bits", [("fp4", 4), ("flint4", 4), ("fp4_er_pos", 4), ("fp4_ea_neg", 4), ("fp3", 3), ("int4", 4),

@@ -278,21 +278,14 @@ def test_a_state_dict_says_its_format(host_linear):
 
 def test_codes_that_the_format_does_not_hold_are_refused():
     """The kernel would keep them within its four bits, which is another weight."""
-    check = packed._check_codes
+    check = packed._check_integers
     for dtype in (torch.int8, torch.uint8):      # bytes, read as the kind's integers
-        check(torch.arange(16).to(dtype), packed.INT_ASYM, None)
-        check(torch.arange(-7, 8).to(torch.int8).view(dtype), packed.INT_SYM, None)
+        check(torch.arange(16).to(dtype), packed.INT_ASYM)
+        check(torch.arange(-7, 8).to(torch.int8).view(dtype), packed.INT_SYM)
         for v, kind in ((16, packed.INT_ASYM), (-1, packed.INT_ASYM), (-128, packed.INT_ASYM), (8, packed.INT_SYM),
                         (-8, packed.INT_SYM), (127, packed.INT_SYM), (-128, packed.INT_SYM)):
             with pytest.raises(ValueError, match="codes"):
-                check(torch.tensor([3, v, 1], dtype=torch.int8).view(dtype), kind, None)
-    values = packed._kind_of(4, "flint4")[1]
-    check(torch.tensor([0, -0.0, 1, -16, 6]).half(), packed.TABLE, values)
-    check(torch.tensor([0, -0.0, 1, -12, 6]).half(), packed.FP4, None)
-    for v, kind in ((5, packed.TABLE), (12, packed.TABLE), (float("nan"), packed.TABLE), (float("inf"), packed.FP4),
-                    (16, packed.FP4), (0.5, packed.FP4), (float("nan"), packed.FP4)):
-        with pytest.raises(ValueError, match="codes"):
-            check(torch.tensor([[1, 2], [v, 0]]).half(), kind, values)
+                check(torch.tensor([3, v, 1], dtype=torch.int8).view(dtype), kind)
 
 
 def test_quant_model_packs_a_shared_layer_in_all_its_places(host_linear):
