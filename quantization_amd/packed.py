@@ -355,6 +355,14 @@ def _workspace(weight, t, code, at, rows, ld, counts, grad):
     return ws, ws.data_ptr(), need
 
 
+def _address(t):
+    """For the library, to which 0 says that there is none."""
+    at = None if t is None else t.data_ptr()
+    if at == 0:
+        raise RuntimeError("a tensor without memory of its own")
+    return at
+
+
 def _forward(x, weight, bias, counts, index):
     L = _bound or _bind()
     (rows, k), code = x.shape, _XDTYPES[x.dtype]
@@ -364,8 +372,7 @@ def _forward(x, weight, bias, counts, index):
         x, ld = (x, k) if x.is_contiguous() else _rows_of(x)
         at = x.data_ptr()
         ws, wp, need = _workspace(weight, x, code, at, rows, ld, counts, 0)
-        rc = L.mq_linear4(ref, at, code, rows, ld, None if bias is None else bias.data_ptr(),
-                          None if counts is None else counts.data_ptr(), y.data_ptr(), wp, need,
+        rc = L.mq_linear4(ref, at, code, rows, ld, _address(bias), _address(counts), y.data_ptr(), wp, need,
                           torch._C._cuda_getCurrentRawStream(index))
         if rc:
             _lib.check(rc)
@@ -383,7 +390,7 @@ def _backward(dy, weight, counts, want_x, want_bias, index):
     dy, ld = _rows_of(dy)
     at, code = dy.data_ptr(), _XDTYPES[dy.dtype]
     ws, wp, need = _workspace(weight, dy, code, at, rows, ld, counts, want_x + 2 * want_bias)
-    rc = L.mq_linear4_grad(ref, at, code, rows, ld, None if counts is None else counts.data_ptr(),
+    rc = L.mq_linear4_grad(ref, at, code, rows, ld, _address(counts),
                            None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), wp, need,
                            torch._C._cuda_getCurrentRawStream(index))
     if rc:

@@ -350,3 +350,20 @@ def test_formats_in_other_clothes(host_linear):
     meta = {k: v.to("meta") for k, v in state.items()}
     m.load_state_dict(meta, assign=True)
     assert m.weight_data.is_meta
+
+
+def test_tensors_without_memory_are_not_taken_for_none(launches):
+    """A wrapper's address is 0, which the library reads as "no bias" and "no counts"."""
+    w = host_weight()
+    e = packed.PackedWeight(w.data, w.params, w.norm, 1, w.n, w.k, w.group_size, w.wq_bits, w.datatype)
+    b, c, y = torch.zeros(w.n, dtype=torch.float16), torch.ones(1, dtype=torch.int32), rows(k=w.n)
+    calls = [(lambda b: run(rows(), w, b), b), (lambda c: run(rows(), e, None, c), c),
+             (lambda c: packed._on_device(packed._backward, y, e, c, True, True), c)]
+    for call, t in calls:
+        call(t)
+        before = len(launches.seen)
+        with pytest.raises(RuntimeError):
+            torch.func.functionalize(call)(t)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(t[None])
+        assert len(launches.seen) == before
